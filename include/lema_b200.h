@@ -311,6 +311,38 @@ int lema_store_exchange_phase(void* table, int64_t cap, int64_t vbytes, const vo
                               int64_t n, int64_t g0, int64_t* counts, uint32_t* status,
                               int64_t seg_groups, int64_t seg_slots, int phase, void* stream);
 
+/*
+ * lema_store_exchange_strided / _seg / _phase on a table whose rows are HELD IN 8 OR 4 BITS: a key's
+ * row (d_v values of `dtype`, LEMA_F32 / LEMA_BF16 / LEMA_F16) is quantised as it is written, and a
+ * found row is given back as the values its codes stand for, in the same dtype; zeros on a miss.
+ *   LEMA_ROWS_INT8  s = fl32(amax / 127) of the row, code = clamp(rne(v / s), -127, 127)
+ *   LEMA_ROWS_FP8   s = the smallest power of two with amax / s <= 448 (2^-126 at least), code = e4m3(v / s)
+ *   LEMA_ROWS_INT4  s = fl32(amax / 7) of each 32 values, code = clamp(rne(v / s), -7, 7)
+ * (rne: the exact quotient rounded, ties to even); the value given back is fl32(s * code), saturated to
+ * dtype's largest finite value, rounded to dtype. An infinity or a NaN makes its scale, and so every value of its group, NaN. A row found
+ * inside the same call (T > 1) is given back as the same numbers a later call would find, so any
+ * chunking of a sequence gives the same results. The table is cap slots of
+ * lema_store_slot_bytes(lema_quant_row_bytes(format, d_v)) bytes, zero-filled before first use.
+ * A held row: codes of ceil(d_v / 8) chunks of 8 values (8 bytes a chunk, low byte first; LEMA_ROWS_INT4:
+ * 4 bytes, low nibble first, two's complement), the fp32 scales, zeros to a multiple of 16 bytes.
+ * heads = 0: item i's rows at i * d_v elements of values and out; heads > 0: the strides (bytes, whole
+ * elements) of lema_store_exchange_strided. phase: 3, or 1 / 2 with T = 1 as lema_store_exchange_phase.
+ * d_v: 1 to 256. Workspace as lema_store_workspace_bytes.
+ * Replaces: code/lema/csrc/store.cpp:127-162 (`exchange`) for quantised rows, which the reference
+ * does not have.
+ */
+#define LEMA_ROWS_INT8 1
+#define LEMA_ROWS_FP8 2
+#define LEMA_ROWS_INT4 3
+int64_t lema_quant_row_bytes(int format, int64_t d_v);   /* 0: unknown format or width */
+int lema_store_exchange_quant(void* table, int64_t cap, int format, int dtype, int64_t d_v,
+                              const void* qcodes, const void* kcodes, int code_bytes,
+                              const void* values, void* out, int64_t n, int64_t T, int64_t g0,
+                              int64_t* counts, uint32_t* status, void* workspace,
+                              size_t workspace_bytes, int64_t seg_groups, int64_t seg_slots,
+                              int64_t heads, int64_t v_sb, int64_t v_sh, int64_t v_st, int64_t o_sb,
+                              int64_t o_sh, int64_t o_st, int phase, void* stream);
+
 /* ----------------------------------- (d) sequence-sharded prefill (config 5) */
 /*
  * One sequence too long for one pass (or one GPU) is cut into contiguous shards of L
@@ -409,6 +441,29 @@ int lema_shard_gather_peer(const int32_t* src, int64_t base, const void* const* 
 int lema_ipc_export(const void* ptr, void* handle, int64_t* offset);
 int lema_ipc_import(const void* handle, int64_t offset, void** ptr);
 int lema_ipc_close(void* ptr, int64_t offset);
+
+/* ------------------------------------------- (e) products with 4-bit weights */
+/*
+ * y[m][n] = sum_k x[m][k] * s[n][k / group] * q[n][k] (+ residual[m][n]), q in -8 ... 7.
+ *   x         [M] rows of K values of `dtype` (LEMA_F32 / LEMA_BF16 / LEMA_F16), ldx elements apart
+ *   packed    ceil(N / 16) x ceil(K / 64) blocks of 16 features x 64 inputs, 512 bytes each: 32 lanes
+ *             (8 a + t: a = feature mod 8, t = 0 .. 3) of four 32-bit words w = 2 h + j; the field of bits
+ *             16 e + 8 p + 4 i ... + 3 of word w holds q + 8 of feature 16 b + 8 i + a (b the block row)
+ *             at input 64 c + 32 h + 8 t + 4 j + 2 p + e (c the block column). Features past N and
+ *             inputs past K hold 8 (a zero weight). 16-byte aligned.
+ *   scales    [ceil(N / 16)][ceil(K / group)][16] of 16 bits (LEMA_BF16 or LEMA_F16: scale_dtype)
+ *   group     32, 64 or 128 inputs a scale; the last one may be short
+ *   residual, y  [M] rows of N values of `dtype`, ldr / ldy elements apart; residual may be NULL or y
+ * gated != 0: the block rows hold 8 gate features (i = 0) and the 8 up features of the same indices
+ * (i = 1), N counts the features of each, and y = silu(gate) * up with both sums in fp32 (ceil(N / 8)
+ * block rows; no residual). Sums are fp32, rounded once to dtype; fp32 inputs keep fp32 accuracy.
+ * Replaces: the nn.Linear layers of code/lema/model.py:85-93, 160-175 and 264 for weights held in 4 bits,
+ * which the reference does not have.
+ */
+int lema_int4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* packed,
+                     const void* scales, int scale_dtype, int group, int64_t N, int gated,
+                     const void* residual, int64_t ldr, void* y, int64_t ldy, uint32_t* status,
+                     void* stream);
 
 #ifdef __cplusplus
 }

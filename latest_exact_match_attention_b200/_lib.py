@@ -50,6 +50,12 @@ _SIGNATURES = {
     "lema_store_exchange_strided": ([_P, _I64, _I64, _P, _P, _I, _P, _P, _I64, _I64, _I64, _P, _P,
                                      _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                      _P], _I),
+    "lema_quant_row_bytes": ([_I, _I64], _I64),
+    "lema_store_exchange_quant": ([_P, _I64, _I, _I, _I64, _P, _P, _I, _P, _P, _I64, _I64, _I64, _P,
+                                   _P, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                   _I, _P], _I),
+    "lema_int4_linear": ([_P, _I, _I64, _I64, _I64, _P, _P, _I, _I, _I64, _I, _P, _I64, _P, _I64, _P,
+                          _P], _I),
     "lema_segment_workspace_bytes": ([_I64, _I64, _I], _SZ),
     "lema_segment_match": ([_P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P, _SZ, _P, _P], _I),
     "lema_lt_table_slots": ([_I64], _I64),

@@ -34,8 +34,9 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import LEMA_STATUS_PROBE_LIMIT, LEMA_STATUS_TABLE_FULL, LemaError, call, ptr, stream_handle
+from ._lib import DTYPE_TAG, LEMA_STATUS_PROBE_LIMIT, LEMA_STATUS_TABLE_FULL, LemaError, call, ptr, stream_handle
 from .attention import code_bytes_of
+from .quant import ROW_FORMATS, dequantize_rows, row_bytes
 
 EMPTY = 0   # state word of a free slot: a zero-filled table is an empty table
 
@@ -68,13 +69,18 @@ class HashStore:
 
     Slot = [code u64 | state u64 | value row] with the row padded to 16 bytes
     (`lema_store_slot_bytes`), so `nbytes()` is cap * slot bytes.
+
+    With `quant` ("int8", "fp8" or "int4") a row is quantised as its key is written and given back
+    as the values it stands for, in `dtype` (`lema_store_exchange_quant`; formats and rounding in
+    include/lema_b200.h): a slot of 24 bf16 values takes 48 or 32 bytes instead of 64.
     """
 
     def __init__(self, d_v: int, groups: int, dtype=torch.bfloat16, capacity: int = 256,
-                 device=None, segments: int = 1):
+                 device=None, segments: int = 1, quant: str | None = None):
         self.dtype = _as_torch_dtype(dtype)
-        self.d_v, self.groups = d_v, groups
-        self.vbytes = d_v * torch.empty((), dtype=self.dtype).element_size()
+        self.d_v, self.groups, self.quant = d_v, groups, quant
+        self.vbytes = (d_v * torch.empty((), dtype=self.dtype).element_size() if quant is None
+                       else row_bytes(quant, d_v))
         if self.vbytes % 8:
             raise ValueError(f"value row of {self.vbytes} bytes breaks slot alignment "
                              f"(d_v * itemsize must be a multiple of 8)")
@@ -140,6 +146,8 @@ class HashStore:
         if values.numel() != n * self.d_v or out.numel() != n * self.d_v or values.shape[-1] != self.d_v:
             raise ValueError(f"values and out must hold [n, d_v] = [{n}, {self.d_v}] rows, got "
                              f"{tuple(values.shape)} and {tuple(out.shape)}")
+        if self.quant is not None:
+            return self._exchange_quant(qcodes, kcodes, values, out, n, T, g0, rows, 3, check)
         if values.element_size() * values.shape[-1] != self.vbytes:
             raise ValueError(f"value rows of {values.element_size() * values.shape[-1]} bytes, "
                              f"the store holds {self.vbytes}")
@@ -161,6 +169,32 @@ class HashStore:
         if check:
             self.check()
 
+    def _exchange_quant(self, qcodes, kcodes, values, out, n, T, g0, rows, phase, check):
+        """lema_store_exchange_quant: `exchange` and `exchange_phase` on quantised rows."""
+        codes = kcodes if qcodes is None else qcodes
+        for t in (values, out):
+            if t is not None and t.dtype != self.dtype:
+                raise ValueError(f"the store quantises {self.dtype} rows, got {t.dtype}")
+        if rows is None:
+            if any(t is not None and t.dim() != 2 for t in (values, out)) or (out is not None and not out.is_contiguous()):
+                raise ValueError("values and out must be [n, d_v] (out contiguous), or pass rows=")
+            values = None if values is None else values.contiguous()
+            rows = (0, 0, 0, 0, 0, 0, 0)
+        cb = code_bytes_of(codes)
+        ws = self._workspace(n, T, cb)
+        qcodes, kcodes = (None if c is None else c.contiguous() for c in (qcodes, kcodes))
+        args = ("lema_store_exchange_quant", ptr(self.table), self.cap, ROW_FORMATS[self.quant],
+                DTYPE_TAG[self.dtype], self.d_v, ptr(qcodes), ptr(kcodes), cb, ptr(values), ptr(out), n, T, g0,
+                ptr(self.counts) + 8 * g0, ptr(self.status), ptr(ws), 0 if ws is None else ws.numel(),
+                self.seg_groups, self.seg_slots, *rows, phase, stream_handle(self.device))
+        if self.device.index in (None, torch.cuda.current_device()):
+            call(*args)
+        else:
+            with torch.cuda.device(self.device):
+                call(*args)
+        if check:
+            self.check()
+
     def exchange_phase(self, qcodes: torch.Tensor, kcodes: torch.Tensor, values: torch.Tensor,
                        out: torch.Tensor, g0: int, phase: int):
         """Half of a decode step's exchange (T = 1, one item per partition): phase 1 looks every
@@ -172,6 +206,13 @@ class HashStore:
         n = codes.numel()
         if g0 < 0 or g0 + n > self.groups:
             raise ValueError(f"groups [{g0}, {g0 + n}) outside the store's {self.groups}")
+        if self.quant is not None:
+            one = phase == 1
+            rows = out if one else values
+            if rows.numel() != n * self.d_v or rows.shape[-1] != self.d_v:
+                raise ValueError(f"rows must be [n, d_v] = [{n}, {self.d_v}], got {tuple(rows.shape)}")
+            return self._exchange_quant(qcodes if one else None, None if one else kcodes, None if one else values,
+                                        out if one else None, n, 1, g0, None, phase, False)
         call("lema_store_exchange_phase", ptr(self.table), self.cap, self.vbytes,
              ptr(qcodes) if phase == 1 else None, ptr(kcodes) if phase == 2 else None,
              code_bytes_of(codes), ptr(values) if phase == 2 else None,
@@ -180,13 +221,15 @@ class HashStore:
 
     def dump(self):
         """Every entry of the store: (groups int64 [n], codes int64 [n], rows [n, d_v] in the
-        store's dtype), in slot order. Codes are the stored 64-bit words (an int32 code's bit
+        store's dtype; of a quantised store the values its rows stand for), in slot order. Codes are the stored 64-bit words (an int32 code's bit
         pattern zero-extended). Reads the table as it is on the device (synchronises)."""
         hdr = self.table.view(-1)[: 16 * self.cap].view(torch.int64).view(self.cap, 2)
         rows = self.table.view(-1)[16 * self.cap:].view(self.cap, self.stride - 16)
         live = (hdr[:, 1] >= 2).nonzero().squeeze(1)
         groups = hdr[live, 1] - 2
         codes = hdr[live, 0]
+        if self.quant is not None:
+            return groups, codes, dequantize_rows(rows[live], self.quant, self.d_v, self.dtype)
         vals = rows[live].view(self.dtype)[:, : self.d_v]
         return groups, codes, vals
 
@@ -312,12 +355,14 @@ class LemaCache:
     max_load, the worst case of one distinct code per token) or `capacity` slots exactly.
     `pin` is accepted for signature compatibility and ignored (nothing crosses the bus).
     `codes_hook(layer, qc, kc) -> (qc, kc)` is applied on the device to every layer's
-    [B, H, T] codes before the exchange.
+    [B, H, T] codes before the exchange. `quant` ("int8", "fp8", "int4") holds the value rows in
+    8 or 4 bits (see HashStore).
     """
 
     def __init__(self, cfg, dtype=torch.bfloat16, pin: bool = True,
                  max_cache_len: int = 8192, max_load: float = 0.7,
-                 batch: int = 1, capacity: int | None = None, codes_hook=None, device=None):
+                 batch: int = 1, capacity: int | None = None, codes_hook=None, device=None,
+                 quant: str | None = None):
         if dtype not in _CARRIER:
             raise ValueError(f"cache dtype must be one of {list(_CARRIER)}, got {dtype}")
         if not 0 < max_load <= 0.95:
@@ -326,7 +371,7 @@ class LemaCache:
         slots = int(capacity) if capacity else math.ceil(cfg.depth * P * max_cache_len / max_load)
         self.cfg, self.batch = cfg, batch
         self.store = HashStore(cfg.d_v, groups=cfg.depth * P, dtype=dtype, capacity=slots,
-                               device=device, segments=cfg.depth)
+                               device=device, segments=cfg.depth, quant=quant)
         self.t = 0
         self.buffers = Buffers(dtype, codes_hook)
         self._views = [LayerStore(self.store, self.buffers, i * P, P) for i in range(cfg.depth)]

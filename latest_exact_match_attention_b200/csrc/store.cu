@@ -39,124 +39,10 @@
 
 #include "common.cuh"
 #include "match.cuh"
+#include "store.cuh"
 
 namespace lema {
 namespace k3 {
-
-constexpr uint64_t kEmpty = 0, kLocked = 1;
-constexpr int kThreads = 256;
-
-struct Args {
-  unsigned char* table;  // the header array
-  unsigned char* rows;   // the row array, table + 16 * cap
-  uint64_t cap;
-  int64_t stride;        // bytes per row in the row array
-  int64_t vbytes;
-  const void* qc;
-  const void* kc;
-  const unsigned char* v;
-  unsigned char* out;
-  int64_t n, T;
-  uint64_t g0;
-  int64_t* counts;
-  uint32_t* status;
-  const int32_t* src;
-  const void* lt_code;
-  const int32_t* lt_pos;
-  const int32_t* lt_count;
-  uint64_t seg_groups;  // > 0: groups [k * seg_groups, (k + 1) * seg_groups) have their home
-  uint64_t seg_slots;   //   slots in [k * seg_slots, (k + 1) * seg_slots); probing still wraps cap
-  // strided value and output rows (heads > 0): item (partition p = b * heads + h, position t)
-  // reads its value row at v + b * v_sb + h * v_sh + t * v_st and writes its output row at
-  // out + b * o_sb + h * o_sh + t * o_st (bytes); heads = 0: rows of item i at i * vbytes
-  int64_t heads, v_sb, v_sh, v_st, o_sb, o_sh, o_st;
-  int phase;  // T == 1: 3 = look up then insert, 1 = look up only, 2 = insert only
-};
-
-__device__ __forceinline__ int64_t row_off(const Args& a, int64_t p, int64_t t, bool out) {
-  if (a.heads == 0) return (p * a.T + t) * a.vbytes;
-  const int64_t b = p / a.heads, h = p - b * a.heads;
-  return out ? b * a.o_sb + h * a.o_sh + t * a.o_st : b * a.v_sb + h * a.v_sh + t * a.v_st;
-}
-template <typename Vec>
-__device__ __forceinline__ const Vec* v_row(const Args& a, int64_t p, int64_t t) {
-  return reinterpret_cast<const Vec*>(a.v + row_off(a, p, t, false));
-}
-template <typename Vec>
-__device__ __forceinline__ Vec* out_row(const Args& a, int64_t p, int64_t t) {
-  return reinterpret_cast<Vec*>(a.out + row_off(a, p, t, true));
-}
-
-// Home slot of (group, code): a 64-bit mix mapped by multiply-high onto the whole table, or,
-// when the table is segmented, onto the group's segment. Probing continues across segment
-// ends and wraps at cap either way, so capacity and fullness are those of one shared table;
-// segmenting only keeps one layer's exchange (its groups) inside a slice of the table.
-__device__ __forceinline__ uint64_t home(uint64_t code, uint64_t group, const Args& a) {
-  const uint64_t h = fmix64(code ^ fmix64(group ^ 0x5851F42D4C957F2Dull));
-  if (a.seg_groups == 0) return __umul64hi(h, a.cap);
-  return (group / a.seg_groups) * a.seg_slots + __umul64hi(h, a.seg_slots);
-}
-
-__device__ __forceinline__ uint64_t ld_acquire(const uint64_t* p) {
-  uint64_t v;
-  asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ void st_release(uint64_t* p, uint64_t v) {
-  asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-
-// Probing is done by a GROUP of kG = 8 lanes per item: each round trip the group reads the
-// next kG consecutive headers (one per lane, 16 bytes each: 128 contiguous bytes) and decides
-// with one ballot which slot, in probe order, ends the probe (its entry, or an empty slot).
-// A chain of c slots then costs about c / 8 dependent round trips instead of c: at load 0.95
-// an unsuccessful linear probe averages ~200 slots. Calls with few items (a batch-1 decode
-// step has 64 per layer) use whole warps instead (kWideG = 32 slots per round trip): the
-// lanes are there for free; mid-sized calls (a batch-256 decode step: 16384 items per layer)
-// use 16 lanes, measured 3.5% faster per step than 32 (fewer waves of warps) and 8% faster
-// than 8 (fewer round trips at load 0.65).
-constexpr int kG = 8;
-constexpr int kWideG = 32;
-constexpr int kMidG = 16;
-constexpr int64_t kWideMaxItems = 4096;   // up to this many items per call: 32-lane groups
-constexpr int64_t kMidMaxItems = 16384;   // up to this many: 16-lane groups
-
-template <int G>
-struct Lane {
-  int j;           // index in the group
-  int gbase;       // the group's first lane in the warp
-  unsigned gmask;  // the group's lanes
-  __device__ __forceinline__ unsigned bits(unsigned ballot) const {
-    return G == 32 ? ballot : (ballot >> gbase) & ((1u << G) - 1u);
-  }
-};
-template <int G>
-__device__ __forceinline__ Lane<G> group_lane() {
-  const int lane = threadIdx.x & 31;
-  const int base = lane & ~(G - 1);
-  return Lane<G>{lane & (G - 1), base, G == 32 ? 0xFFFFFFFFu : (((1u << G) - 1u) << base)};
-}
-
-__device__ __forceinline__ uint64_t wrap_add(uint64_t s, uint64_t d, uint64_t cap) {
-  s += d;
-  while (s >= cap) s -= cap;
-  return s;
-}
-
-__device__ __forceinline__ uint64_t* header(const Args& a, uint64_t s) {
-  return reinterpret_cast<uint64_t*>(a.table) + 2 * s;
-}
-template <typename Vec>
-__device__ __forceinline__ Vec* row_of(const Args& a, uint64_t s) {
-  return reinterpret_cast<Vec*>(a.rows + s * a.stride);
-}
-// (code, state) of slot s, through L2: other items of the same launch may claim slots of it
-__device__ __forceinline__ void read_header(const Args& a, uint64_t s, uint64_t& code, uint64_t& state) {
-  const ulonglong2 h = __ldcg(reinterpret_cast<const ulonglong2*>(header(a, s)));
-  code = h.x;
-  state = h.y;
-}
 
 // The group's lanes copy / zero the row's vector words j, j + G, ...
 template <int G, typename Vec>
@@ -460,6 +346,44 @@ WsLayout layout(int64_t n, int64_t T, int code_bytes) {
   return w;
 }
 
+int chunk_match(Args& a, void* ws, size_t ws_bytes, int code_bytes, cudaStream_t stream) {
+  const WsLayout w = layout(a.n, a.T, code_bytes);
+  unsigned char* base = static_cast<unsigned char*>(ws);
+  MatchLaunch m;
+  m.qc = a.qc;
+  m.kc = a.kc;
+  m.code_bytes = code_bytes;
+  m.N = a.n / a.T;
+  m.T = a.T;
+  m.src = reinterpret_cast<int32_t*>(base + w.src);
+  m.lt_code = base + w.lt_code;
+  m.lt_pos = reinterpret_cast<int32_t*>(base + w.lt_pos);
+  m.lt_count = reinterpret_cast<int32_t*>(base + w.lt_count);
+  m.ws = (ws_bytes > w.match) ? base + w.match : nullptr;
+  m.ws_bytes = ws_bytes - w.match;
+  m.status = a.status;
+  m.stream = stream;
+  LEMA_TRY(launch_match(m));
+  a.src = m.src;
+  a.lt_code = m.lt_code;
+  a.lt_pos = m.lt_pos;
+  a.lt_count = m.lt_count;
+  return LEMA_OK;
+}
+
+int group_lanes(int64_t n) {
+  // LEMA_K3_WIDE_MAX overrides the item count up to which 32-lane groups probe (same results)
+  int64_t wide_max = kWideMaxItems;
+  if (const char* e = std::getenv("LEMA_K3_WIDE_MAX")) wide_max = std::atoll(e);
+  int G = n <= wide_max ? kWideG : (n <= kMidMaxItems ? kMidG : kG);
+  // LEMA_K3_GROUP=8/16/32 sets the lanes per item for every call (same results)
+  if (const char* e = std::getenv("LEMA_K3_GROUP")) {
+    const int g = std::atoi(e);
+    if (g == 8 || g == 16 || g == 32) G = g;
+  }
+  return G;
+}
+
 // LEMA_K3_INTERLEAVE=0 runs a decode step's lookup and insert probes one after the other
 // (exchange_step) instead of interleaved (exchange_both); the same results either way.
 inline bool interleave() {
@@ -477,28 +401,7 @@ int run(Args a, int64_t T, void* ws, size_t ws_bytes, int code_bytes, cudaStream
       LEMA_CUDA_TRY(launch_dependent(exchange_step<CodeT, Vec, G>, dim3(blocks), dim3(kThreads), 0, stream, a));
     return LEMA_OK;
   }
-  const WsLayout w = layout(a.n, T, code_bytes);
-  unsigned char* base = static_cast<unsigned char*>(ws);
-  MatchLaunch m;
-  m.qc = a.qc;
-  m.kc = a.kc;
-  m.code_bytes = code_bytes;
-  m.N = a.n / T;
-  m.T = T;
-  m.src = reinterpret_cast<int32_t*>(base + w.src);
-  m.lt_code = base + w.lt_code;
-  m.lt_pos = reinterpret_cast<int32_t*>(base + w.lt_pos);
-  m.lt_count = reinterpret_cast<int32_t*>(base + w.lt_count);
-  m.ws = (ws_bytes > w.match) ? base + w.match : nullptr;
-  m.ws_bytes = ws_bytes - w.match;
-  m.status = a.status;
-  m.stream = stream;
-  const int rc = launch_match(m);
-  if (rc != LEMA_OK) return rc;
-  a.src = m.src;
-  a.lt_code = m.lt_code;
-  a.lt_pos = m.lt_pos;
-  a.lt_count = m.lt_count;
+  LEMA_TRY(chunk_match(a, ws, ws_bytes, code_bytes, stream));
   LEMA_CUDA_TRY(launch_dependent(exchange_resolve<CodeT, Vec, G>, dim3(blocks), dim3(kThreads), 0, stream, a));
   LEMA_CUDA_TRY(launch_dependent(exchange_insert<CodeT, Vec, G>, dim3(blocks), dim3(kThreads), 0, stream, a));
   return LEMA_OK;
@@ -590,15 +493,7 @@ int store_exchange(void* table, int64_t cap, int64_t vbytes, const void* qc, con
   a.seg_slots = static_cast<uint64_t>(seg_slots);
   const uint64_t st = rows ? static_cast<uint64_t>(rows[1] | rows[2] | rows[3] | rows[4] | rows[5] | rows[6]) : 0;
   const bool v16 = vbytes % 16 == 0 && st % 16 == 0 && aligned(values, 16) && aligned(out, 16);
-  // LEMA_K3_WIDE_MAX overrides the item count up to which 32-lane groups probe (same results)
-  int64_t wide_max = k3::kWideMaxItems;
-  if (const char* e = std::getenv("LEMA_K3_WIDE_MAX")) wide_max = std::atoll(e);
-  int G = n <= wide_max ? k3::kWideG : (n <= k3::kMidMaxItems ? k3::kMidG : k3::kG);
-  // LEMA_K3_GROUP=8/16/32 sets the lanes per item for every call (same results)
-  if (const char* e = std::getenv("LEMA_K3_GROUP")) {
-    const int g = std::atoi(e);
-    if (g == 8 || g == 16 || g == 32) G = g;
-  }
+  const int G = k3::group_lanes(n);
   if (code_bytes == 4) {
     if (v16) return k3::run_g<uint32_t, uint4>(G, a, T, ws, ws_bytes, code_bytes, stream);
     return k3::run_g<uint32_t, uint2>(G, a, T, ws, ws_bytes, code_bytes, stream);

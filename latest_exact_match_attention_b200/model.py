@@ -31,6 +31,7 @@ from torch import nn
 from . import _lib
 from ._lib import DTYPE_TAG, call, check_status, device_status, ptr, stream_handle
 from .attention import pack_codes, prefill_match, proj_codes
+from .quant import Int4Linear, Int4SwiGLU
 
 ATTN_KINDS = ("lema",)
 
@@ -272,6 +273,9 @@ class Block(nn.Module):
         B, H, T, dv = got.shape
         dim = x.shape[-1]
         y = got.transpose(1, 2).reshape(B * T, H * dv)
+        if isinstance(self.attn.o_proj, Int4Linear):
+            x = self.attn.o_proj(y, x.reshape(B * T, dim)).view(B, T, dim)
+            return self.mlp(rms_norm(self.norm2, x), residual=x)
         x = torch.addmm(x.reshape(B * T, dim), y, self.attn.o_proj.weight.t()).view(B, T, dim)
         return self.mlp(rms_norm(self.norm2, x), residual=x)
 
@@ -318,7 +322,8 @@ class Transformer(nn.Module):
         """The retrieval cache for this model, in device memory (the store is HBM-resident;
         place "ram" is accepted for the reference's call sites and means the same).
         Keywords as code/lema/cache.py:313-355: max_cache_len= or capacity=, max_load=,
-        batch=, dtype= (default: the model's), codes_hook=."""
+        batch=, dtype= (default: the model's), codes_hook=; and quant= ("int8", "fp8", "int4")
+        for value rows held in 8 or 4 bits."""
         from .cache import LemaCache
         if place not in ("hbm", "vram", "ram"):
             raise ValueError(f"place must be 'hbm' (or 'ram'/'vram', the same device store), "
@@ -344,6 +349,21 @@ class Transformer(nn.Module):
         # raised here, once per forward, outside graph capture
         check_status(x.device, "Transformer.forward")
         return out
+
+    @torch.no_grad()
+    def quantize_weights_(self, group: int = 128) -> "Transformer":
+        """Replaces, in place, the value and output projections, the MLPs and the head by 4-bit
+        weights with one scale per `group` inputs (round to nearest, `quant.quantize_weight`): what
+        a decode step reads of them falls to about a quarter. q_proj and k_proj keep their type:
+        an exact match needs every sign of a code, and rounding their weights flips signs.
+        The model's parameters (and its caches' dtype) keep theirs; state dicts of a quantised model
+        load into a model quantised with the same group."""
+        for b in self.blocks:
+            b.attn.v_proj = Int4Linear.from_linear(b.attn.v_proj, group)
+            b.attn.o_proj = Int4Linear.from_linear(b.attn.o_proj, group)
+            b.mlp = Int4SwiGLU.from_mlp(b.mlp, group)
+        self.lm_head = Int4Linear.from_linear(self.lm_head, group)
+        return self
 
     def n_params(self, embedding: bool = True) -> int:
         """Parameter count; embedding=False leaves out the token embedding and the head."""
