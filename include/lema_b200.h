@@ -451,12 +451,16 @@ int lema_ipc_close(void* ptr, int64_t offset);
  *             16 e + 8 p + 4 i ... + 3 of word w holds q + 8 of feature 16 b + 8 i + a (b the block row)
  *             at input 64 c + 32 h + 8 t + 4 j + 2 p + e (c the block column). Features past N and
  *             inputs past K hold 8 (a zero weight). 16-byte aligned.
- *   scales    [ceil(N / 16)][ceil(K / group)][16] of 16 bits (LEMA_BF16 or LEMA_F16: scale_dtype)
+ *   scales    [ceil(N / 16)][ceil(K / group)][8][2] of 16 bits (LEMA_BF16 or LEMA_F16: scale_dtype): [b][.][a][i]
+ *             of feature 16 b + 8 i + a. 4-byte aligned.
  *   group     32, 64 or 128 inputs a scale; the last one may be short
  *   residual, y  [M] rows of N values of `dtype`, ldr / ldy elements apart; residual may be NULL or y
  * gated != 0: the block rows hold 8 gate features (i = 0) and the 8 up features of the same indices
  * (i = 1), N counts the features of each, and y = silu(gate) * up with both sums in fp32 (ceil(N / 8)
- * block rows; no residual). Sums are fp32, rounded once to dtype; fp32 inputs keep fp32 accuracy.
+ * block rows; no residual). Sums are fp32, rounded once to dtype; fp32 inputs keep fp32 accuracy. Up to 32
+ * rows, and rows that TMA cannot read (K < 64, ldx or x not a multiple of 16 bytes), multiply the codes
+ * exactly and scale each group's fp32 sum; more 16-bit rows multiply s * q rounded once to dtype.
+ * Device-side conditions (a bounded wait that ran out) are OR-ed into status.
  * Replaces: the nn.Linear layers of code/lema/model.py:85-93, 160-175 and 264 for weights held in 4 bits,
  * which the reference does not have.
  */

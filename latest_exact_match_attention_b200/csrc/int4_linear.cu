@@ -20,65 +20,13 @@
 
 #include <algorithm>
 
-#include "common.cuh"
+#include "int4.cuh"
 
 namespace lema {
 namespace w4 {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-
-struct Args {
-  const uint4* w;           // [n_rb][n_kb][32]
-  const uint16_t* scales;   // [n_rb][n_groups][16]
-  const void* x;
-  const void* r;
-  void* y;
-  int64_t ldx, ldr, ldy;    // elements
-  int64_t M;
-  int K, N;                 // inputs, output features
-  int n_rb, n_kb, n_groups;
-  int log_group;            // 5, 6 or 7
-  int scale_bf16;
-  int vec;                  // x rows readable in whole aligned chunks of 8 values
-};
-
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-
-__device__ __forceinline__ float scale_of(uint16_t bits, int bf16) {
-  return bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
-}
-
-// Four pairs of weights of one word as 16-bit floats of type T (the A fragment of one K16 step).
-template <typename T> struct Unpack;
-template <> struct Unpack<__nv_bfloat16> {
-  __device__ static __forceinline__ void run(uint32_t w, uint32_t (&a)[4]) {
-    const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t u = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;  // 128 + u
-      const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);
-      a[j] = *reinterpret_cast<const uint32_t*>(&v);
-    }
-  }
-};
-template <> struct Unpack<__half> {
-  __device__ static __forceinline__ void run(uint32_t w, uint32_t (&a)[4]) {
-    const __half2 off = __floats2half2_rn(1032.f, 1032.f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t u = ((w >> (4 * j)) & 0x000F000Fu) | 0x64006400u;  // 1024 + u
-      const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), off);
-      a[j] = *reinterpret_cast<const uint32_t*>(&v);
-    }
-  }
-};
-template <> struct Unpack<float> : Unpack<__nv_bfloat16> {};
+constexpr int64_t kMaxRows = 32;  // more rows go to the tcgen05 kernel where it can read x
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -149,9 +97,6 @@ __device__ __forceinline__ void load_x(const float* row, int k, int K, int vec, 
   }
 }
 
-// silu(g) * u in fp32.
-__device__ __forceinline__ float gate_up(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-
 // kNT token tiles of 8 rows and kR block rows of 16 features a CTA.
 template <typename T, int kNT, int kR, bool kGated>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const Args a) {
@@ -212,8 +157,8 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Args a) {
               for (int q = 0; q < Parts<T>::kN; ++q) mma<T>(part[n], f, b[n][q][2 * j], b[n][q][2 * j + 1]);
           }
           const int rb = min(rb0 + r, a.n_rb - 1);
-          const uint16_t* sc = a.scales + (static_cast<int64_t>(rb) * a.n_groups + grp) * 16;
-          const float s0 = scale_of(__ldg(sc + g), a.scale_bf16), s1 = scale_of(__ldg(sc + g + 8), a.scale_bf16);
+          const uint32_t two = __ldg(reinterpret_cast<const uint32_t*>(a.scales) + (static_cast<int64_t>(rb) * a.n_groups + grp) * 8 + g);
+          const float s0 = scale_of(static_cast<uint16_t>(two), a.scale_bf16), s1 = scale_of(static_cast<uint16_t>(two >> 16), a.scale_bf16);
 #pragma unroll
           for (int n = 0; n < kNT; ++n) {
             acc[r][n][0] = fmaf(s0, part[n][0], acc[r][n][0]);
@@ -294,7 +239,6 @@ extern "C" int lema_int4_linear(const void* x, int dtype, int64_t M, int64_t K, 
                                 void* stream) {
   using namespace lema;
   clear_error();
-  (void)status;
   if (dtype != LEMA_F32 && dtype != LEMA_BF16 && dtype != LEMA_F16) return fail(LEMA_ERR_INVALID_ARGUMENT, "int4_linear: dtype tag %d", dtype);
   if (scale_dtype != LEMA_BF16 && scale_dtype != LEMA_F16) return fail(LEMA_ERR_INVALID_ARGUMENT, "int4_linear: scales are bf16 or fp16 (dtype tag %d)", scale_dtype);
   if (group != 32 && group != 64 && group != 128) return fail(LEMA_ERR_INVALID_ARGUMENT, "int4_linear: a scale covers 32, 64 or 128 inputs, got %d", group);
@@ -307,8 +251,8 @@ extern "C" int lema_int4_linear(const void* x, int dtype, int64_t M, int64_t K, 
   if (M == 0) return LEMA_OK;
   if (x == nullptr || packed == nullptr || scales == nullptr || y == nullptr) return fail(LEMA_ERR_INVALID_ARGUMENT, "int4_linear: null pointer");
   const int64_t es = dtype == LEMA_F32 ? 4 : 2;
-  if (!aligned(packed, 16) || !aligned(scales, 2) || !aligned(x, es) || !aligned(y, es) || !aligned(residual, es))
-    return fail(LEMA_ERR_INVALID_ARGUMENT, "int4_linear: packed weights must be 16-byte aligned, the others to their elements");
+  if (!aligned(packed, 16) || !aligned(scales, 4) || !aligned(x, es) || !aligned(y, es) || !aligned(residual, es))
+    return fail(LEMA_ERR_INVALID_ARGUMENT, "int4_linear: packed weights must be 16-byte aligned, scales 4, the others to their elements");
   const DeviceInfo* dev = current_device_info();
   if (dev == nullptr) return LEMA_ERR_CUDA;
   if (dev->cc_major != 10) return fail(LEMA_ERR_UNSUPPORTED, "built for sm_100a; device is sm_%d%d", dev->cc_major, dev->cc_minor);
@@ -331,6 +275,7 @@ extern "C" int lema_int4_linear(const void* x, int dtype, int64_t M, int64_t K, 
   a.scale_bf16 = scale_dtype == LEMA_BF16;
   a.vec = aligned(x, 16) && (M == 1 || (ldx * es) % 16 == 0);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M > w4::kMaxRows && w4::tile_ok(a, dtype)) return w4::run_tile(a, dtype, gated != 0, status, s);
   if (dtype == LEMA_F32) return w4::run_rows<float>(a, gated != 0, s);
   if (dtype == LEMA_BF16) return w4::run_rows<__nv_bfloat16>(a, gated != 0, s);
   return w4::run_rows<__half>(a, gated != 0, s);

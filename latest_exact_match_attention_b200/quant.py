@@ -74,7 +74,7 @@ def _check_codes(codes: torch.Tensor, scales: torch.Tensor, group: int):
 
 class Int4Weight:
     """A [n, k] weight (gated: a gate and an up weight of n features each) in the kernel's layout:
-    `packed` int32 [block rows, block columns, 32, 4] and `scales` [block rows, groups, 16]."""
+    `packed` int32 [block rows, block columns, 32, 4] and `scales` [block rows, groups, 8, 2]."""
 
     __slots__ = ("packed", "scales", "n", "k", "group", "gated")
 
@@ -83,7 +83,7 @@ class Int4Weight:
         per = 8 if gated else 16
         rb = -(-n // per)
         if group not in GROUPS or packed.dtype != torch.int32 or scales.dtype not in (torch.bfloat16, torch.float16) \
-                or tuple(packed.shape) != (rb, -(-k // 64), 32, 4) or tuple(scales.shape) != (rb, -(-k // group), 16) \
+                or tuple(packed.shape) != (rb, -(-k // 64), 32, 4) or tuple(scales.shape) != (rb, -(-k // group), 8, 2) \
                 or not packed.is_contiguous() or not scales.is_contiguous() or packed.device != scales.device:
             raise ValueError(f"not a packed 4-bit weight of {n} x {k}, group {group}: packed {packed.dtype} "
                              f"{tuple(packed.shape)}, scales {scales.dtype} {tuple(scales.shape)}")
@@ -115,7 +115,7 @@ class Int4Weight:
         u = u.view(rb, 2, 8, kp // 64, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1).to(torch.int32)
         shift = torch.arange(8, device=u.device, dtype=torch.int32) * 4         # bits 16 e + 8 p + 4 i
         words = (u.reshape(rb, kp // 64, 8, 4, 2, 2, 8) << shift).sum(-1, dtype=torch.int32)
-        return Int4Weight(words.view(rb, kp // 64, 32, 4).contiguous(), s.transpose(1, 2).contiguous(), n, k, group, gated)
+        return Int4Weight(words.view(rb, kp // 64, 32, 4).contiguous(), s.unflatten(1, (2, 8)).permute(0, 3, 2, 1).contiguous(), n, k, group, gated)
 
     def codes(self):
         """The codes int8 and scales as packed: [n, k], [n, groups] (gated: a pair of them)."""
@@ -123,7 +123,7 @@ class Int4Weight:
         shift = torch.arange(8, device=self.packed.device, dtype=torch.int32) * 4
         u = ((self.packed.view(rb, kb, 8, 4, 2, 2, 1) >> shift) & 15).view(rb, kb, 8, 4, 2, 2, 2, 2, 2)
         u = u.permute(0, 8, 2, 1, 4, 3, 5, 7, 6).reshape(rb, 16, kb * 64)[..., : self.k]
-        q, s = (u - 8).to(torch.int8), self.scales.transpose(1, 2)
+        q, s = (u - 8).to(torch.int8), self.scales.permute(0, 3, 2, 1).flatten(1, 2)
         if not self.gated:
             return q.reshape(-1, self.k)[: self.n], s.reshape(rb * 16, -1)[: self.n]
         return tuple((q[:, i:i + 8].reshape(-1, self.k)[: self.n], s[:, i:i + 8].reshape(rb * 8, -1)[: self.n])
