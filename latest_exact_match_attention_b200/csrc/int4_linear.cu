@@ -101,6 +101,7 @@ __device__ __forceinline__ void load_x(const float* row, int k, int K, int vec, 
 template <typename T, int kNT, int kR, bool kGated>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const Args a) {
   __shared__ float4 sums[kWarps][kR][kNT][32];
+  griddep_launch();
   griddep_wait();  // launched as a dependent: x and the residual first
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;

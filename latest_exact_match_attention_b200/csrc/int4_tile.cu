@@ -35,13 +35,15 @@ constexpr int kSetWarps = 4;
 constexpr int kMine = kTileBlocks / kSetWarps;    // block rows a warp
 constexpr int kTileThreads = 32 * (6 + kSets * kSetWarps);
 
+// Room for tiles of up to BN tokens. Clusters that split K (BN = 64 only) add the sums they receive.
 template <int BN>
 struct Tile {
-  static constexpr int kBBytes = BN * kBK * 2;
-  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStageBytes = kABytes + BN * kBK * 2;
   static constexpr int kStages = BN == 64 ? 8 : 4;
   static constexpr uint32_t kTmemCols = 2 * BN;
-  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + 1024 /* alignment */ + 512 /* barriers */;
+  static constexpr int kUnitBytes = 8 * kTileRows * 4;  // 8 tokens of a tile's sums
+  static constexpr int kRecvBytes = BN == 64 ? 7 * kUnitBytes : 0;
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kRecvBytes + 1024 /* alignment */ + 512 /* barriers */;
 };
 
 struct TileArgs {
@@ -50,6 +52,8 @@ struct TileArgs {
   uint64_t wait_ns;
   int64_t n_tiles;
   int f_tiles;       // tiles along the weight rows
+  int bn;            // tokens a tile, a multiple of 32
+  int split;         // CTAs of a cluster that share a tile's K (1: none)
   int pairs;         // rows of y and of the residual hold whole aligned pairs of features
 };
 
@@ -99,8 +103,107 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xFFFFFFFFu, wait_phase(bar, parity, abort_flag, status, wait_ns));
 }
 
+__device__ __forceinline__ bool warp_ready(uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity)); }
+
 __device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
   mma_bf16(d_tmem, a_desc, b_desc, idesc, acc);  // kind::f16; the types are the descriptor's
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// 16 bytes into the shared memory of CTA `rank` of the cluster, at this CTA's address `addr`.
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, float a, float b, float c, float d) {
+  uint32_t to;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+// silu(g) * u with approximate exponential and reciprocal: within 2^-17 of the value for |g| < 87 (the exponent's
+// product is off by half a unit in its last place, |g| 2^-24 of it), far inside the 16-bit rounding that follows;
+// below -87 zero, where silu is under 2^-119. The exact quotient's slow path kept the epilogue behind the tiles:
+// 8192 rows, 2 x 4096 x 1536: 287 -> 214 us.
+__device__ __forceinline__ float gate_up_fast(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+
+// A fragment's row g lies at row slot(g) of its 8 rows of the A operand: with consecutive g four rows apart, the eight
+// lanes of one write phase (two g, four chunks each) cover all banks of the swizzled rows. row_of(slot(g)) == g.
+__device__ __forceinline__ int slot_of(int g) { return ((g & 1) << 2) | (g >> 1); }
+__device__ __forceinline__ int row_of(int slot) { return ((slot & 3) << 1) | (slot >> 2); }
+
+// The outputs of kCols tokens of this lane's weight row, from their fp32 sums: residual or activation, one
+// rounding, stores. m: the first token.
+template <typename T, bool kGated, int kCols>
+__device__ __forceinline__ void finish(const TileArgs& p, int row, int64_t m, const float (&r)[kCols]) {
+  const Args& a = p.a;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kCols), a.M - m));  // tokens there are
+  // lanes l and l ^ 4 hold two adjacent features; the first finishes both for one token of a pair, the second for
+  // the other, so that outputs and residual move in 32-bit words where rows allow it
+  const int odd = (row >> 2) & 1;
+  float v[kGated ? kCols / 4 : kCols / 2][2];
+  int f, step, first;  // v[i]: features f, f + 1 of token first + i * step
+  if constexpr (kGated) {
+    // block rows hold 8 gate rows, then the 8 up rows of the same features: lanes l and l ^ 8 swap one
+    // value of each pair of tokens, and each applies the activation to one token
+    const bool gate = (row & 8) == 0;
+    float act[kCols / 2];
+#pragma unroll
+    for (int c = 0; c < kCols / 2; ++c) {
+      const float other = __shfl_xor_sync(0xFFFFFFFFu, gate ? r[2 * c + 1] : r[2 * c], 8);
+      act[c] = gate_up_fast(gate ? r[2 * c] : other, gate ? other : r[2 * c + 1]);
+    }
+#pragma unroll
+    for (int c = 0; c < kCols / 4; ++c) {
+      const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? act[2 * c] : act[2 * c + 1], 4);
+      v[c][0] = odd ? other : act[2 * c];
+      v[c][1] = odd ? act[2 * c + 1] : other;
+    }
+    f = (row >> 4) * 8 + 2 * (row & 3);
+    step = 4;
+    first = 2 * odd + (gate ? 0 : 1);
+  } else {
+#pragma unroll
+    for (int c = 0; c < kCols / 2; ++c) {
+      const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? r[2 * c] : r[2 * c + 1], 4);
+      v[c][0] = odd ? other : r[2 * c];
+      v[c][1] = odd ? r[2 * c + 1] : other;
+    }
+    f = (row & ~7) + 2 * (row & 3);
+    step = 2;
+    first = odd;
+  }
+  constexpr int kN = kGated ? kCols / 4 : kCols / 2;
+  if (f >= a.N) return;
+  T* y = static_cast<T*>(a.y) + (m + first) * a.ldy + f;
+  const T* res = kGated || a.r == nullptr ? nullptr : static_cast<const T*>(a.r) + (m + first) * a.ldr + f;
+  const int64_t dy = step * a.ldy, dr = step * a.ldr;
+  if (p.pairs) {
+    if (res != nullptr) {
+      uint32_t rs[kN];  // all of them in flight before the first store
+#pragma unroll
+      for (int i = 0; i < kN; ++i) rs[i] = first + i * step < rows ? *reinterpret_cast<const uint32_t*>(res + i * dr) : 0u;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float2 add = Pair<T>::to_f2(rs[i]);
+        v[i][0] += add.x;
+        v[i][1] += add.y;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (first + i * step < rows) *reinterpret_cast<uint32_t*>(y + i * dy) = Pair<T>::from_f(v[i][0], v[i][1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      if (first + i * step >= rows) continue;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (f + e < a.N) y[i * dy + e] = from_f<T>(v[i][e] + (res != nullptr ? to_f(res[i * dr + e]) : 0.f));
+    }
+  }
 }
 
 template <typename T, int BN, bool kGated, bool kSame>
@@ -110,13 +213,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   // instruction descriptor (tcgen05.mma kind::f16): fp32 accumulator, A and B of type T (0 fp16, 1 bf16), both
   // K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
   constexpr uint32_t kType = Pair<T>::kBf16;
-  constexpr uint32_t kInstrDesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
+  const uint32_t instr_desc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(p.bn >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
   static_assert(kStages % kSets == 0 && kTileBlocks % kSetWarps == 0, "whole shares");
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);
   unsigned char* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
   const uint32_t sbase = smem_addr(smem);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  const uint32_t recv = sbase + kStages * kStageBytes;  // sums of other CTAs of a split tile
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes + TL::kRecvBytes);
   // barriers: x full, weights full, empty [kStages each], acc_full[2], acc_empty[2], drain
   const uint32_t bar0 = smem_addr(bars);
   auto xfull_bar = [&](int s) { return bar0 + 8u * s; };
@@ -130,6 +234,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
 
   const Args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // this CTA's tiles, and its share of their K blocks
+  // (grid: x the CTAs of a cluster, y the tiles; read as blockIdx and gridDim everywhere, which keeps the loops'
+  // counters and the MMA's descriptors in uniform registers: copies of them cost 8% at 16384 rows)
+  const int split = BN == 64 ? p.split : 1, rank = BN == 64 ? static_cast<int>(blockIdx.x) : 0;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * a.n_kb / split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * a.n_kb / split);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(xfull_bar(s), 1);
@@ -155,6 +265,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
+  if (split > 1) cluster_arrive();  // answered before the first store into another CTA
+  griddep_launch();
   griddep_wait();  // launched as a dependent: x and the residual are read only from here on
 
   if (warp == 0) {
@@ -163,14 +275,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
       int s = 0;
       uint32_t ph = 0, issued = 0, last_ph = 0;
       bool ok = true;
-      for (int64_t tile = blockIdx.x; ok && tile < p.n_tiles; tile += gridDim.x) {
-        const int m0 = static_cast<int>(tile / p.f_tiles) * BN;
-        for (int kb = 0; kb < a.n_kb; ++kb) {
+      for (int64_t tile = blockIdx.y; ok && tile < p.n_tiles; tile += gridDim.y) {
+        const int m0 = static_cast<int>(tile / p.f_tiles) * p.bn;
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!wait_phase(empty_bar(s), ph ^ 1u, s_abort, p.status, p.wait_ns)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(xfull_bar(s), TL::kBBytes);
+          mbar_arrive_expect_tx(xfull_bar(s), static_cast<uint32_t>(p.bn * kBK * 2));
           tma_load_2d(sbase + s * kStageBytes + kABytes, &map_x, xfull_bar(s), kb * kBK, m0);
           issued |= 1u << s;
           last_ph = (last_ph & ~(1u << s)) | (ph << s);
@@ -191,11 +303,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
       int s = 0, acc = 0;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
-      for (int64_t tile = blockIdx.x; ok && tile < p.n_tiles; tile += gridDim.x) {
+      for (int64_t tile = blockIdx.y; ok && tile < p.n_tiles; tile += gridDim.y) {
         if (!wait_phase(acce_bar(acc), aph ^ 1u, s_abort, p.status, p.wait_ns)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-        for (int kb = 0; kb < a.n_kb; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!wait_phase(xfull_bar(s), ph, s_abort, p.status, p.wait_ns) ||
               !wait_phase(wfull_bar(s), ph, s_abort, p.status, p.wait_ns)) {
             ok = false;
@@ -206,7 +318,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
           const uint64_t a_desc = sw128_desc(a_addr), b_desc = sw128_desc(a_addr + kABytes);
 #pragma unroll
           for (int kk = 0; kk < kBK / 16; ++kk)
-            mma_16bit(d_tmem, a_desc + 2u * kk, b_desc + 2u * kk, kInstrDesc, (kb | kk) != 0 ? 1u : 0u);
+            mma_16bit(d_tmem, a_desc + 2u * kk, b_desc + 2u * kk, instr_desc, (kb - kb0) | kk ? 1u : 0u);
           mma_commit(empty_bar(s));
           if (++s == kStages) {
             s = 0;
@@ -228,76 +340,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;  // a warp reads TMEM lanes 32 * (warp % 4) ... + 31
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const T* res = static_cast<const T*>(a.r);
-    T* y = static_cast<T*>(a.y);
     int acc = 0;
     uint32_t aph = 0;
-    for (int64_t tile = blockIdx.x; tile < p.n_tiles; tile += gridDim.x) {
+    for (int64_t tile = blockIdx.y; split == 1 && tile < p.n_tiles; tile += gridDim.y) {
       if (!warp_wait(accf_bar(acc), aph, s_abort, p.status, p.wait_ns)) break;
       tc_fence_after();
-      const int64_t m0 = (tile / p.f_tiles) * BN;
+      const int64_t m0 = (tile / p.f_tiles) * p.bn;
       const int row = static_cast<int>(tile % p.f_tiles) * kTileRows + quarter * 32 + lane;  // weight row
-      for (int j = 0; j < BN / 32; ++j) {
-        const int64_t m = m0 + j * 32;
+      for (int j = 0; j < p.bn; j += 32) {
+        const int64_t m = m0 + j;
         if (m >= a.M) break;  // warp-uniform
         uint32_t r[32];
-        tmem_load32(tmem_base + lane_base + static_cast<uint32_t>(acc * BN + j * 32), r);
-        if constexpr (kGated) {
-          // block rows hold 8 gate rows, then the 8 up rows of the same features: lanes l and l ^ 8 swap one
-          // value of each pair of tokens, and each finishes one token
-          const bool gate = (row & 8) == 0;
-          const int f = (row >> 4) * 8 + (row & 7);
+        tmem_load32(tmem_base + lane_base + static_cast<uint32_t>(acc * BN + j), r);
+        float v[32];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const float even = __uint_as_float(r[c]), odd = __uint_as_float(r[c + 1]);
-            const float other = __shfl_xor_sync(0xFFFFFFFFu, gate ? odd : even, 8);
-            const float v = gate ? gate_up(even, other) : gate_up(other, odd);
-            const int64_t t = m + c + (gate ? 0 : 1);
-            if (f < a.N && t < a.M) y[t * a.ldy + f] = from_f<T>(v);
-          }
-        } else {
-          // lanes l and l ^ 1 swap one value of each pair of tokens: each finishes two features of one token,
-          // so that residual and output move in 32-bit words where rows allow it
-          const int odd = lane & 1, f = row & ~1;
-          float v[16][2];
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float lo = __uint_as_float(r[2 * c]), hi = __uint_as_float(r[2 * c + 1]);
-            const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? lo : hi, 1);
-            v[c][0] = odd ? other : lo;
-            v[c][1] = odd ? hi : other;
-          }
-          if (p.pairs) {
-            if (res != nullptr) {
-              uint32_t rs[16];  // all of them in flight before the first store
-#pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                const int64_t t = m + 2 * c + odd;
-                rs[c] = f < a.N && t < a.M ? *reinterpret_cast<const uint32_t*>(res + t * a.ldr + f) : 0u;
-              }
-#pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                const float2 add = Pair<T>::to_f2(rs[c]);
-                v[c][0] += add.x;
-                v[c][1] += add.y;
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const int64_t t = m + 2 * c + odd;
-              if (f < a.N && t < a.M) *reinterpret_cast<uint32_t*>(y + t * a.ldy + f) = Pair<T>::from_f(v[c][0], v[c][1]);
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const int64_t t = m + 2 * c + odd;
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (f + e < a.N && t < a.M)
-                  y[t * a.ldy + f + e] = from_f<T>(v[c][e] + (res != nullptr ? to_f(res[t * a.ldr + f + e]) : 0.f));
-            }
-          }
-        }
+        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(r[c]);
+        finish<T, kGated, 32>(p, row, m, v);
       }
       tc_fence_before();
       __syncwarp();
@@ -310,15 +368,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
   } else {
     // ------------------------------------------------------------ dequantisation
     const int set = (warp - 6) / kSetWarps, blk0 = (warp - 6) % kSetWarps * kMine, g = lane >> 2, t = lane & 3;
-    // Odd rows take their upper half first: the eight lanes of one write phase then cover all banks.
-    const bool odd = g & 1;
     // row r's 16-byte chunk c lies at r * 128 + ((c ^ (r & 7)) << 4) of the stage
-    const uint32_t row0 = (blk0 * 16 + g) * 128;
-    const uint32_t c0 = row0 + (((odd ? 4 : 0) + t) ^ g) * 16, c1 = row0 + (((odd ? 0 : 4) + t) ^ g) * 16;
+    const uint32_t row0 = (blk0 * 16 + slot_of(g)) * 128;
+    const uint32_t c0 = row0 + (t ^ slot_of(g)) * 16, c1 = row0 + ((4 + t) ^ slot_of(g)) * 16;
     const int sc_second = a.log_group == 5 ? 8 : 0;  // to the upper half's scales
-    int s = set, skip = set;  // skip: stages until this set's next one
+    int s = set, skip = kb0 + set;  // skip: the place along K of this set's next stage
     uint32_t ph = 1;
-    for (int64_t tile = blockIdx.x; tile < p.n_tiles; tile += gridDim.x) {
+    for (int64_t tile = blockIdx.y; tile < p.n_tiles; tile += gridDim.y) {
       const int rb0 = static_cast<int>(tile % p.f_tiles) * kTileBlocks + blk0;
       const uint4* wp[kMine];
       const uint32_t* sp[kMine];
@@ -336,13 +392,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
 #pragma unroll
         for (int b = 0; b < kMine; ++b) {
           next[b] = __ldg(wp[b] + kb * 32);
-          next_sc[b][0] = __ldg(sp[b] + grp * 8);
-          next_sc[b][1] = __ldg(sp[b] + grp * 8 + up);
+          next_sc[b][0] = next_sc[b][1] = __ldg(sp[b] + grp * 8);
+          if (up != 0) next_sc[b][1] = __ldg(sp[b] + grp * 8 + up);
         }
       };
       int kb = skip;
-      if (kb < a.n_kb) fetch(kb);
-      for (; kb < a.n_kb; kb += kSets) {
+      if (kb < kb1) fetch(kb);
+      for (; kb < kb1; kb += kSets) {
         uint4 w[kMine];
         uint32_t sc[kMine][2];
 #pragma unroll
@@ -351,13 +407,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
           sc[b][0] = next_sc[b][0];
           sc[b][1] = next_sc[b][1];
         }
-        if (kb + kSets < a.n_kb) fetch(kb + kSets);
+        fetch(min(kb + kSets, kb1 - 1));
         unsigned char* dst = smem + s * kStageBytes;
 #pragma unroll
         for (int b = 0; b < kMine; ++b) {
-          uint4 v[2][2];  // [row g / g + 8][first or second half written]: 8 consecutive inputs each
-          const uint32_t words[4] = {odd ? w[b].z : w[b].x, odd ? w[b].w : w[b].y, odd ? w[b].x : w[b].z, odd ? w[b].y : w[b].w};
-          const uint32_t two[2] = {odd ? sc[b][1] : sc[b][0], odd ? sc[b][0] : sc[b][1]};
+          uint4 v[2][2];  // [row g / g + 8][half]: 8 consecutive inputs each
+          const uint32_t words[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t f0[4], f1[4];
@@ -365,14 +420,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             Unpack<T>::run(words[2 * h + 1], f1);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const RowScale<T, kSame> rs(two[h], i, a.scale_bf16);
+              const RowScale<T, kSame> rs(sc[b][h], i, a.scale_bf16);
               v[i][h].x = rs.times(f0[i]);
               v[i][h].y = rs.times(f0[i + 2]);
               v[i][h].z = rs.times(f1[i]);
               v[i][h].w = rs.times(f1[i + 2]);
             }
           }
-          if (b == 0 && !warp_wait(empty_bar(s), ph, s_abort, p.status, p.wait_ns)) goto done;
+          if (b == 0 && !warp_ready(empty_bar(s), ph) && !warp_wait(empty_bar(s), ph, s_abort, p.status, p.wait_ns)) goto done;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             *reinterpret_cast<uint4*>(dst + c0 + b * 2048 + i * 1024) = v[i][0];
@@ -388,9 +443,76 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
           ph ^= 1u;
         }
       }
-      skip = kb - a.n_kb;
+      skip = kb - kb1 + kb0;
     }
   done:;
+  }
+
+  if constexpr (BN == 64) {
+    if (split > 1) {
+      // One tile a cluster: CTA q of it finishes units u = q, q + split, ... of 8 tokens. Every CTA sends its sums
+      // of the others' units, all meet, and the sums are added in the order of the ranks.
+      const int64_t m0 = static_cast<int64_t>(blockIdx.y / p.f_tiles) * p.bn;
+      const int quarter = warp & 3, row_in = quarter * 32 + lane;
+      const int row = static_cast<int>(blockIdx.y % p.f_tiles) * kTileRows + row_in;
+      const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+      const bool live = warp >= 2 && warp < 6;
+      const int slots = (p.bn / 8 + split - 1) / split;  // units of one CTA
+      // where source q's sums of my unit k lie: [q or q - 1][k][two halves of 4 tokens][128 rows]
+      auto place = [&](int src, int dst, int k) {
+        return recv + static_cast<uint32_t>(((src < dst ? src : src - 1) * slots + k) * TL::kUnitBytes + row_in * 16);
+      };
+      bool ok = false;
+      cluster_wait();
+      if (live) {
+        ok = warp_wait(accf_bar(0), 0, s_abort, p.status, p.wait_ns);
+        tc_fence_after();
+        for (int u = 0; u < p.bn / 8; ++u) {
+          const int to = u % split;
+          if (to == rank || m0 + u * 8 >= a.M || !ok) continue;  // warp-uniform
+          uint32_t r[8];
+          tmem_load8(tmem_base + lane_base + static_cast<uint32_t>(u * 8), r);
+          const uint32_t at = place(rank, to, u / split);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            store_remote(at + h * (TL::kUnitBytes / 2), to, __uint_as_float(r[4 * h]), __uint_as_float(r[4 * h + 1]),
+                         __uint_as_float(r[4 * h + 2]), __uint_as_float(r[4 * h + 3]));
+        }
+      }
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      if (live && ok) {
+        for (int k = 0; k < slots; ++k) {
+          const int u = k * split + rank;
+          if (u * 8 >= p.bn || m0 + u * 8 >= a.M) break;  // warp-uniform
+          uint32_t r[8];
+          tmem_load8(tmem_base + lane_base + static_cast<uint32_t>(u * 8), r);
+          float v[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = 0.f;
+          for (int q = 0; q < split; ++q) {
+            if (q == rank) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c) v[c] += __uint_as_float(r[c]);
+              continue;
+            }
+            const uint32_t at = place(q, rank, k);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float f[4];
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
+                           : "r"(at + h * (TL::kUnitBytes / 2))
+                           : "memory");
+#pragma unroll
+              for (int c = 0; c < 4; ++c) v[4 * h + c] += f[c];
+            }
+          }
+          finish<T, kGated, 8>(p, row, m0 + u * 8, v);
+        }
+      }
+    }
   }
 
   tc_fence_before();
@@ -406,25 +528,65 @@ bool tile_ok(const Args& a, int dtype) {
 }
 
 template <typename T, int BN, bool kGated, bool kSame>
-int launch_tile(const CUtensorMap& map, const TileArgs& p, int64_t grid, cudaStream_t stream) {
+int launch_tile(const CUtensorMap& map, const TileArgs& p, int grid, cudaStream_t stream) {
   const auto kernel = tile_kernel<T, BN, kGated, kSame>;
   LEMA_TRY(kernel_facts(reinterpret_cast<const void*>(kernel), Tile<BN>::kSmemBytes, 0, 0, nullptr));
-  LEMA_CUDA_TRY(launch_dependent(kernel, dim3(static_cast<unsigned>(grid)), dim3(kTileThreads), Tile<BN>::kSmemBytes, stream, map, p));
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(static_cast<unsigned>(p.split), static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = Tile<BN>::kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  if (pdl_enabled()) {  // a dependent launch, see common.cuh
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.split > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  LEMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, p));
   return LEMA_OK;
 }
 
 template <typename T, int BN>
-int launch_width(const CUtensorMap& map, const TileArgs& p, int64_t grid, bool gated, cudaStream_t stream) {
+int launch_width(const CUtensorMap& map, const TileArgs& p, int grid, bool gated, cudaStream_t stream) {
   const bool same = p.a.scale_bf16 == Pair<T>::kBf16;
   if (gated) return same ? launch_tile<T, BN, true, true>(map, p, grid, stream) : launch_tile<T, BN, true, false>(map, p, grid, stream);
   return same ? launch_tile<T, BN, false, true>(map, p, grid, stream) : launch_tile<T, BN, false, false>(map, p, grid, stream);
 }
 
 template <typename T>
-int launch_type(int bn, const CUtensorMap& map, const TileArgs& p, int64_t grid, bool gated, cudaStream_t stream) {
-  if (bn == 64) return launch_width<T, 64>(map, p, grid, gated, stream);
-  if (bn == 128) return launch_width<T, 128>(map, p, grid, gated, stream);
+int launch_type(const CUtensorMap& map, const TileArgs& p, int grid, bool gated, cudaStream_t stream) {
+  if (p.bn <= 64) return launch_width<T, 64>(map, p, grid, gated, stream);
+  if (p.bn <= 128) return launch_width<T, 128>(map, p, grid, gated, stream);
   return launch_width<T, 256>(map, p, grid, gated, stream);
+}
+
+// The tile width and the split of K with the least estimated time: rounds of tiles over the SMs, each of
+// n_kb / split stages that cost the tensor cores 2 cycles a token and the dequantising warps about 400 cycles,
+// and a fixed part (filling the ring, the last epilogue; a split's exchange).
+void choose_shape(TileArgs& p, int sms) {
+  double best = 0;
+  for (int bn = 32; bn <= 256; bn += 32) {
+    if (bn > 64 && bn - 32 >= p.a.M) break;  // wider than the rows there are
+    const int64_t tiles = ((p.a.M + bn - 1) / bn) * p.f_tiles;
+    for (int split : {1, 2, 3, 4, 8}) {
+      if (split > 1 && (bn > 64 || tiles * split > sms || p.a.n_kb < 4 * split)) continue;
+      const double rounds = static_cast<double>((tiles * split + sms - 1) / sms);
+      const double stage = std::max(400.0, 2.0 * bn) + 0.4 * std::min(400.0, 2.0 * bn);
+      const double cost = rounds * ((p.a.n_kb + split - 1) / split) * stage + 10.0 * bn + (split > 1 ? 2500 : 0);
+      if (best == 0 || cost < best) {
+        best = cost;
+        p.bn = bn;
+        p.split = split;
+        p.n_tiles = tiles;
+      }
+    }
+  }
 }
 
 int run_tile(const Args& a, int dtype, bool gated, uint32_t* status, cudaStream_t stream) {
@@ -438,17 +600,14 @@ int run_tile(const Args& a, int dtype, bool gated, uint32_t* status, cudaStream_
   p.wait_ns = wait_limit_ns();
   p.f_tiles = (a.n_rb + kTileBlocks - 1) / kTileBlocks;
   p.pairs = a.N % 2 == 0 && a.ldy % 2 == 0 && aligned(a.y, 4) && (a.r == nullptr || (a.ldr % 2 == 0 && aligned(a.r, 4)));
-  // the widest tile that still gives every SM a tile
-  int bn = 256;
-  while (bn > 64 && (a.M <= bn / 2 || ((a.M + bn - 1) / bn) * p.f_tiles < dev->sms)) bn /= 2;
-  p.n_tiles = ((a.M + bn - 1) / bn) * p.f_tiles;
+  choose_shape(p, dev->sms);
   CUtensorMap map;
-  if (!encode_kmajor(enc, &map, a.x, a.M, a.K, a.ldx, bn,
+  if (!encode_kmajor(enc, &map, a.x, a.M, a.K, a.ldx, p.bn,
                      dtype == LEMA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16))
     return fail(LEMA_ERR_INVALID_ARGUMENT, "int4_linear: tensor map encoding failed (M=%lld K=%d ldx=%lld)", (long long)a.M, a.K, (long long)a.ldx);
-  const int64_t grid = std::min<int64_t>(p.n_tiles, dev->sms);
-  if (dtype == LEMA_BF16) return launch_type<__nv_bfloat16>(bn, map, p, grid, gated, stream);
-  return launch_type<__half>(bn, map, p, grid, gated, stream);
+  const int grid = static_cast<int>(std::min<int64_t>(p.n_tiles, dev->sms));
+  if (dtype == LEMA_BF16) return launch_type<__nv_bfloat16>(map, p, grid, gated, stream);
+  return launch_type<__half>(map, p, grid, gated, stream);
 }
 
 }  // namespace w4
