@@ -12,20 +12,27 @@
 // tensor cores in fp32 from exact integers; only then the group's sum is scaled, in fp32: no weight is
 // rounded. fp32 inputs are cut into three bf16 parts of 8 significant bits each (exactly their 24),
 // multiplied in turn into the same sums.
-// A CTA of 8 warps holds a few block rows; the warps take the K blocks in turn and their sums meet in
-// shared memory, in the warps' order: results do not depend on timing.
+// A warp holds kR block rows and every KS-th block of K; the KS warps of the same block rows lie in one CTA and
+// their sums meet in shared memory, added in the warps' order: results do not depend on timing. KS is chosen
+// so that the card is full of warps: a token through a 1536 x 1536 projection has 96 block rows and takes 16
+// warps for each, the vocabulary's 3144 block rows one each. What bounds the small calls is the latency of a
+// few dependent loads, so every warp keeps kDeep blocks (words, scales and inputs) in flight in registers; the large
+// ones are bound by the instructions issued, about 70 a block of 1024 weights where rows are whole (kWhole: K a
+// multiple of 64, 16-byte aligned rows, so that no load is checked; rows past the last read the last again, and
+// what they give is dropped). A ring in shared memory (cp.async) instead of registers was no faster.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "int4.cuh"
 
 namespace lema {
 namespace w4 {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kWarps = 8, kMaxSplit = 16;  // warps of a CTA (or as many as share a block row), and of a block row
 constexpr int64_t kMaxRows = 32;  // more rows go to the tcgen05 kernel where it can read x
 
 template <typename T>
@@ -49,33 +56,65 @@ __device__ __forceinline__ void mma<float>(float (&c)[4], const uint32_t (&a)[4]
   mma<__nv_bfloat16>(c, a, b0, b1);
 }
 
-// 8 consecutive inputs as packed pairs: one part for 16-bit rows, three bf16 parts for fp32 rows.
-template <typename T> struct Parts { static constexpr int kN = 1; };
-template <> struct Parts<float> { static constexpr int kN = 3; };
-
+// The first product of a sum: c = a b.
 template <typename T>
-__device__ __forceinline__ void load_x(const T* row, int k, int K, int vec, uint32_t (&b)[1][4]) {
-  if (vec && k + 8 <= K) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + k));
-    b[0][0] = v.x; b[0][1] = v.y; b[0][2] = v.z; b[0][3] = v.w;
-  } else {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(row) + k;
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_first<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <>
+__device__ __forceinline__ void mma_first<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <>
+__device__ __forceinline__ void mma_first<float>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  mma_first<__nv_bfloat16>(c, a, b0, b1);
+}
+
+// 8 consecutive inputs of one row as they lie in memory, zeros past the row's end.
+template <typename T>
+struct Raw {
+  uint32_t v[2 * sizeof(T)];
+  __device__ __forceinline__ void load_whole(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = k + 2 * i < K ? h[2 * i] : 0, hi = k + 2 * i + 1 < K ? h[2 * i + 1] : 0;
-      b[0][i] = lo | (hi << 16);
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
     }
   }
-}
-__device__ __forceinline__ void load_x(const float* row, int k, int K, int vec, uint32_t (&b)[3][4]) {
-  float f[8];
-  if (vec && k + 8 <= K) {
-    const float4 u = __ldg(reinterpret_cast<const float4*>(row + k)), v = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
-    f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
-  } else {
+  __device__ __forceinline__ void load(const T* p, int k, int K, int vec) {  // p: input k
+    if (vec && k + 8 <= K) {
+      load_whole(p);
+    } else if constexpr (sizeof(T) == 2) {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = k + i < K ? row[k + i] : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = k + 2 * i < K ? h[2 * i] : 0, hi = k + 2 * i + 1 < K ? h[2 * i + 1] : 0;
+        v[i] = lo | (hi << 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = k + i < K ? __float_as_uint(p[i]) : 0u;
+    }
   }
+};
+
+// The B fragments they make: four pairs of 16-bit values; one part for 16-bit rows, three bf16 parts for fp32 rows.
+template <typename T> struct Parts { static constexpr int kN = 1; };
+template <> struct Parts<float> { static constexpr int kN = 3; };
+template <typename T>
+__device__ __forceinline__ void cut(const Raw<T>& r, uint32_t (&b)[1][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[0][i] = r.v[i];
+}
+__device__ __forceinline__ void cut(const Raw<float>& r, uint32_t (&b)[3][4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t p[3][2];
@@ -83,8 +122,8 @@ __device__ __forceinline__ void load_x(const float* row, int k, int K, int vec, 
     for (int e = 0; e < 2; ++e) {
       // the upper 16 bits are a bf16 with 8 of the 24 significant bits; what is left is exact.
       // An infinity or a NaN goes into the first part alone (a NaN as a quiet one).
-      float v = f[2 * i + e];
-      const bool finite = (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u;
+      float v = __uint_as_float(r.v[2 * i + e]);
+      const bool finite = (r.v[2 * i + e] & 0x7F800000u) != 0x7F800000u;
       if (v != v) v = __uint_as_float(0x7FC00000u);
 #pragma unroll
       for (int q = 0; q < 3; ++q) {
@@ -97,138 +136,210 @@ __device__ __forceinline__ void load_x(const float* row, int k, int K, int vec, 
   }
 }
 
-// kNT token tiles of 8 rows and kR block rows of 16 features a CTA.
-template <typename T, int kNT, int kR, bool kGated>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const Args a) {
-  __shared__ float4 sums[kWarps][kR][kNT][32];
-  griddep_launch();
-  griddep_wait();  // launched as a dependent: x and the residual first
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int rb0 = blockIdx.x * kR;
-  const T* x = static_cast<const T*>(a.x);
-  const int64_t m_tiles = (a.M + 8 * kNT - 1) / (8 * kNT);
-  for (int64_t mt = blockIdx.y; mt < m_tiles; mt += gridDim.y) {
-    const int64_t m0 = mt * (8 * kNT);
-    float acc[kR][kNT][4];
+// How blocks are read: kWhole, kWholeHalf (a scale covers 32 inputs, half a block): rows whole (see above) and scales
+// of the rows' own 16-bit type (bf16 for fp32 rows). kAny: everything else, checked.
+enum Mode { kWhole, kWholeHalf, kAny };
+
+// kNT token tiles of 8 rows and one block row of 16 features a warp.
+template <typename T, int kNT, bool kGated, Mode kMode>
+struct Rows {
+  static constexpr bool kChecked = kMode == kAny;
+  static constexpr int kGroups = kMode == kWhole ? 1 : 2;  // scales of a block
+  static constexpr int kDeep = kNT == 4 || (sizeof(T) == 4 && kNT == 2) ? 1 : (sizeof(T) == 4 ? 2 : 4);
+
+  struct Block {
+    uint4 w;
+    uint32_t s[kGroups];  // rows g (low half) and g + 8
+    Raw<T> x[kNT][2];
+  };
+  // Where a lane reads next: words and scales of block row rb, 2 x 8 inputs of rows m + 8 n + g.
+  struct Source {
+    const uint4* w;
+    const uint32_t* s;
+    const T* x[kNT];
+    int kb;
+  };
+  __device__ static __forceinline__ Source source(const Args& a, int rb, int64_t m, int kb, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    Source src;
+    src.w = a.w + (static_cast<int64_t>(rb) * a.n_kb + kb) * 32 + lane;
+    src.s = reinterpret_cast<const uint32_t*>(a.scales) + static_cast<int64_t>(rb) * a.n_groups * 8 + g;
 #pragma unroll
-    for (int r = 0; r < kR; ++r)
+    for (int n = 0; n < kNT; ++n)  // a row past the last is the last again
+      src.x[n] = static_cast<const T*>(a.x) + min(m + 8 * n + g, a.M - 1) * a.ldx + kb * 64 + 8 * t;
+    src.kb = kb;
+    return src;
+  }
+  // The next block, `split` blocks of K apart.
+  __device__ static __forceinline__ void load(Block& b, const Args& a, Source& src, int split, int lane) {
+    b.w = __ldg(src.w);
 #pragma unroll
-      for (int n = 0; n < kNT; ++n)
+    for (int h = 0; h < kGroups; ++h) {
+      int grp = (src.kb * 64 + 32 * h) >> a.log_group;
+      if (kChecked) grp = min(grp, a.n_groups - 1);
+      b.s[h] = __ldg(src.s + grp * 8);
+    }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][n][c] = 0.f;
-    for (int kb = warp; kb < a.n_kb; kb += kWarps) {
-      uint4 w[kR];
-#pragma unroll
-      for (int r = 0; r < kR; ++r)
-        w[r] = rb0 + r < a.n_rb ? __ldg(a.w + (static_cast<int64_t>(rb0 + r) * a.n_kb + kb) * 32 + lane)
-                                : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+    for (int n = 0; n < kNT; ++n) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = kb * 64 + h * 32 + t * 8;
-        uint32_t b[kNT][Parts<T>::kN][4];
+        if constexpr (kChecked)
+          b.x[n][h].load(src.x[n] + 32 * h, src.kb * 64 + 32 * h + 8 * (lane & 3), a.K, a.vec);
+        else
+          b.x[n][h].load_whole(src.x[n] + 32 * h);
+      }
+      src.x[n] += 64 * split;
+    }
+    src.w += 32 * split;
+    src.kb += split;
+  }
+
+  __device__ static __forceinline__ float scale(uint32_t two, int hi, const Args& a) {
+    const uint16_t bits = static_cast<uint16_t>(hi ? two >> 16 : two);
+    return scale_of(bits, kChecked ? a.scale_bf16 : !std::is_same<T, __half>::value);
+  }
+  __device__ static __forceinline__ void add(const Block& b, const Args& a, float (&acc)[kNT][4]) {
+    float part[kNT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t x[kNT][Parts<T>::kN][4];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) cut(b.x[n][h], x[n]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t f[4];
+        Unpack<T>::run(h == 0 ? (j == 0 ? b.w.x : b.w.y) : (j == 0 ? b.w.z : b.w.w), f);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int q = 0; q < Parts<T>::kN; ++q) {
+            if (j == 0 && q == 0 && (kGroups == 2 || h == 0))
+              mma_first<T>(part[n], f, x[n][q][2 * j], x[n][q][2 * j + 1]);
+            else
+              mma<T>(part[n], f, x[n][q][2 * j], x[n][q][2 * j + 1]);
+          }
+      }
+      if (kGroups == 2 || h == 1) {
+        const uint32_t two = b.s[kGroups == 2 ? h : 0];
+        const float s0 = scale(two, 0, a), s1 = scale(two, 1, a);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
-          const int64_t m = m0 + n * 8 + g;
-          if (m < a.M) {
-            load_x(x + m * a.ldx, k, a.K, a.vec, b[n]);
-          } else {
-#pragma unroll
-            for (int q = 0; q < Parts<T>::kN; ++q)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) b[n][q][i] = 0;
-          }
-        }
-        const int grp = min((kb * 64 + h * 32) >> a.log_group, a.n_groups - 1);
-#pragma unroll
-        for (int r = 0; r < kR; ++r) {
-          const uint32_t* words = reinterpret_cast<const uint32_t*>(&w[r]);
-          float part[kNT][4];
-#pragma unroll
-          for (int n = 0; n < kNT; ++n)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) part[n][c] = 0.f;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t f[4];
-            Unpack<T>::run(words[2 * h + j], f);
-#pragma unroll
-            for (int n = 0; n < kNT; ++n)
-#pragma unroll
-              for (int q = 0; q < Parts<T>::kN; ++q) mma<T>(part[n], f, b[n][q][2 * j], b[n][q][2 * j + 1]);
-          }
-          const int rb = min(rb0 + r, a.n_rb - 1);
-          const uint32_t two = __ldg(reinterpret_cast<const uint32_t*>(a.scales) + (static_cast<int64_t>(rb) * a.n_groups + grp) * 8 + g);
-          const float s0 = scale_of(static_cast<uint16_t>(two), a.scale_bf16), s1 = scale_of(static_cast<uint16_t>(two >> 16), a.scale_bf16);
-#pragma unroll
-          for (int n = 0; n < kNT; ++n) {
-            acc[r][n][0] = fmaf(s0, part[n][0], acc[r][n][0]);
-            acc[r][n][1] = fmaf(s0, part[n][1], acc[r][n][1]);
-            acc[r][n][2] = fmaf(s1, part[n][2], acc[r][n][2]);
-            acc[r][n][3] = fmaf(s1, part[n][3], acc[r][n][3]);
-          }
-        }
-      }
-    }
-    __syncthreads();  // the previous tile's sums have been read
-#pragma unroll
-    for (int r = 0; r < kR; ++r)
-#pragma unroll
-      for (int n = 0; n < kNT; ++n)
-        sums[warp][r][n][lane] = make_float4(acc[r][n][0], acc[r][n][1], acc[r][n][2], acc[r][n][3]);
-    __syncthreads();
-    // each thread finishes the four outputs (features i, i + 8; rows 2 t, 2 t + 1) of a lane
-    for (int i = threadIdx.x; i < kR * kNT * 32; i += kThreads) {
-      const int l = i & 31, n = (i >> 5) % kNT, r = (i >> 5) / kNT;
-      float4 s = sums[0][r][n][l];
-#pragma unroll
-      for (int q = 1; q < kWarps; ++q) {
-        const float4 o = sums[q][r][n][l];
-        s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
-      }
-      const int rb = rb0 + r;
-      if (rb >= a.n_rb) continue;
-      const int64_t m = m0 + n * 8 + 2 * (l & 3);
-      T* y = static_cast<T*>(a.y);
-      if constexpr (kGated) {
-        const int f = rb * 8 + (l >> 2);
-        if (f < a.N) {
-          if (m < a.M) y[m * a.ldy + f] = from_f<T>(gate_up(s.x, s.z));
-          if (m + 1 < a.M) y[(m + 1) * a.ldy + f] = from_f<T>(gate_up(s.y, s.w));
-        }
-      } else {
-        const T* res = static_cast<const T*>(a.r);
-        const float v[2][2] = {{s.x, s.y}, {s.z, s.w}};
-#pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2) {
-          const int f = rb * 16 + (l >> 2) + 8 * i2;
-          if (f >= a.N) continue;
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (m + e < a.M)
-              y[(m + e) * a.ldy + f] = from_f<T>(v[i2][e] + (res != nullptr ? to_f(res[(m + e) * a.ldr + f]) : 0.f));
+          acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
+          acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
+          acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
+          acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
         }
       }
     }
   }
+
+  // The four outputs of lane l's sums s: features of rows l / 4 and l / 4 + 8 of block row rb, rows m + 2 (l % 4), + 1.
+  __device__ static __forceinline__ void finish(const Args& a, int rb, int64_t m, int l, const float4& s) {
+    if (rb >= a.n_rb) return;
+    m += 2 * (l & 3);
+    T* y = static_cast<T*>(a.y);
+    if constexpr (kGated) {
+      const int f = rb * 8 + (l >> 2);
+      if (f >= a.N) return;
+      if (m < a.M) y[m * a.ldy + f] = from_f<T>(gate_up(s.x, s.z));
+      if (m + 1 < a.M) y[(m + 1) * a.ldy + f] = from_f<T>(gate_up(s.y, s.w));
+    } else {
+      const T* res = static_cast<const T*>(a.r);
+      const float v[2][2] = {{s.x, s.y}, {s.z, s.w}};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int f = rb * 16 + (l >> 2) + 8 * i;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (f < a.N && m + e < a.M)
+            y[(m + e) * a.ldy + f] = from_f<T>(v[i][e] + (res != nullptr ? to_f(res[(m + e) * a.ldr + f]) : 0.f));
+      }
+    }
+  }
+};
+
+template <typename T, int kNT, bool kGated, Mode kMode>
+__global__ void __launch_bounds__(32 * kMaxSplit) rows_kernel(const Args a, int split) {
+  using R = Rows<T, kNT, kGated, kMode>;
+  __shared__ float4 sums[kMaxSplit][kNT][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rb = blockIdx.x * ((blockDim.x >> 5) / split) + warp / split, first = warp % split;
+  griddep_launch();
+  if (rb < a.n_rb && first < a.n_kb)  // while the previous kernel ends (a hint: it reads nothing)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + (static_cast<int64_t>(rb) * a.n_kb + first) * 32 + lane));
+  griddep_wait();  // launched as a dependent: x and the residual first
+  const int64_t m_tiles = (a.M + 8 * kNT - 1) / (8 * kNT);
+#pragma unroll 1
+  for (int64_t mt = blockIdx.y; mt < m_tiles; mt += gridDim.y) {
+    const int64_t m0 = mt * (8 * kNT);
+    float acc[kNT][4];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[n][c] = 0.f;
+    if (rb < a.n_rb) {
+      typename R::Block blk[R::kDeep];
+      typename R::Source src = R::source(a, rb, m0, first, lane);
+#pragma unroll
+      for (int u = 0; u < R::kDeep; ++u)
+        if (src.kb < a.n_kb) R::load(blk[u], a, src, split, lane);
+#pragma unroll 1
+      for (int kb = first; kb < a.n_kb;) {
+#pragma unroll
+        for (int u = 0; u < R::kDeep; ++u, kb += split) {
+          if (kb >= a.n_kb) break;
+          R::add(blk[u], a, acc);
+          if (src.kb < a.n_kb) R::load(blk[u], a, src, split, lane);
+        }
+      }
+    }
+    if (split == 1) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) R::finish(a, rb, m0 + 8 * n, lane, make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]));
+      continue;
+    }
+    __syncthreads();  // the previous tile's sums have been read
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) sums[warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+    __syncthreads();
+    // the split warps of a block row share its token tiles
+    for (int n = first; n < kNT; n += split) {
+      const int w0 = warp - first;
+      float4 s = sums[w0][n][lane];
+      for (int q = 1; q < split; ++q) {
+        const float4 o = sums[w0 + q][n][lane];
+        s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+      }
+      R::finish(a, rb, m0 + 8 * n, lane, s);
+    }
+  }
 }
 
-template <typename T, int kNT, int kR>
-int launch_rows(const Args& a, bool gated, cudaStream_t stream) {
+template <typename T, int kNT>
+int launch_rows(const Args& a, bool gated, int sms, cudaStream_t stream) {
+  // warps a block row: up to about 24 on every SM, and a block of K for each
+  int split = 1;
+  while (split < kMaxSplit && static_cast<int64_t>(a.n_rb) * split * 2 <= 24 * static_cast<int64_t>(sms) && 2 * split <= a.n_kb) split *= 2;
+  const int warps = std::max(kWarps, split), per_cta = warps / split;
   const int64_t tiles = (a.M + 8 * kNT - 1) / (8 * kNT);
-  const dim3 grid(static_cast<unsigned>((a.n_rb + kR - 1) / kR), static_cast<unsigned>(std::min<int64_t>(tiles, 65535)));
-  if (gated)
-    LEMA_CUDA_TRY(launch_dependent(rows_kernel<T, kNT, kR, true>, grid, dim3(kThreads), 0, stream, a));
-  else
-    LEMA_CUDA_TRY(launch_dependent(rows_kernel<T, kNT, kR, false>, grid, dim3(kThreads), 0, stream, a));
-  return LEMA_OK;
+  const dim3 grid(static_cast<unsigned>((a.n_rb + per_cta - 1) / per_cta), static_cast<unsigned>(std::min<int64_t>(tiles, 65535)));
+  const dim3 block(static_cast<unsigned>(32 * warps));
+  const bool whole = a.vec && a.K % 64 == 0 && a.scale_bf16 == !std::is_same<T, __half>::value;
+  const auto go = [&](auto kernel) {
+    LEMA_CUDA_TRY(launch_dependent(kernel, grid, block, 0, stream, a, split));
+    return static_cast<int>(LEMA_OK);
+  };
+  if (!whole) return gated ? go(rows_kernel<T, kNT, true, kAny>) : go(rows_kernel<T, kNT, false, kAny>);
+  if (a.log_group == 5) return gated ? go(rows_kernel<T, kNT, true, kWholeHalf>) : go(rows_kernel<T, kNT, false, kWholeHalf>);
+  return gated ? go(rows_kernel<T, kNT, true, kWhole>) : go(rows_kernel<T, kNT, false, kWhole>);
 }
 
 template <typename T>
-int run_rows(const Args& a, bool gated, cudaStream_t stream) {
-  if (a.M <= 8) return launch_rows<T, 1, 1>(a, gated, stream);
-  if (a.M <= 16) return launch_rows<T, 2, 1>(a, gated, stream);
-  return launch_rows<T, 4, 1>(a, gated, stream);
+int run_rows(const Args& a, bool gated, int sms, cudaStream_t stream) {
+  if (a.M <= 8) return launch_rows<T, 1>(a, gated, sms, stream);
+  if constexpr (sizeof(T) == 2)
+    if (a.M > 16) return launch_rows<T, 4>(a, gated, sms, stream);
+  return launch_rows<T, 2>(a, gated, sms, stream);
 }
 
 }  // namespace w4
@@ -277,7 +388,7 @@ extern "C" int lema_int4_linear(const void* x, int dtype, int64_t M, int64_t K, 
   a.vec = aligned(x, 16) && (M == 1 || (ldx * es) % 16 == 0);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (M > w4::kMaxRows && w4::tile_ok(a, dtype)) return w4::run_tile(a, dtype, gated != 0, status, s);
-  if (dtype == LEMA_F32) return w4::run_rows<float>(a, gated != 0, s);
-  if (dtype == LEMA_BF16) return w4::run_rows<__nv_bfloat16>(a, gated != 0, s);
-  return w4::run_rows<__half>(a, gated != 0, s);
+  if (dtype == LEMA_F32) return w4::run_rows<float>(a, gated != 0, dev->sms, s);
+  if (dtype == LEMA_BF16) return w4::run_rows<__nv_bfloat16>(a, gated != 0, dev->sms, s);
+  return w4::run_rows<__half>(a, gated != 0, dev->sms, s);
 }

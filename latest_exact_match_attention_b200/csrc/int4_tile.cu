@@ -566,27 +566,36 @@ int launch_type(const CUtensorMap& map, const TileArgs& p, int grid, bool gated,
   return launch_width<T, 256>(map, p, grid, gated, stream);
 }
 
-// The tile width and the split of K with the least estimated time: rounds of tiles over the SMs, each of
-// n_kb / split stages that cost the tensor cores 2 cycles a token and the dequantising warps about 400 cycles,
-// and a fixed part (filling the ring, the last epilogue; a split's exchange).
-void choose_shape(TileArgs& p, int sms) {
+// The tile width and the split of K with the least estimated time (us): rounds of tiles over the SMs, or of
+// clusters over what can be resident at once, each of n_kb / split stages of 0.36 (the dequantising warps', up to 128
+// tokens) to 0.42 (256 tokens), and a fixed part: filling the ring, the last epilogue, a split's exchange. Measured,
+// 1536 x 4096: 64 rows split 8 ways 9.6, not split 28; 256 rows as 96 CTAs split 2 ways 17.7, as 144 CTAs split 3
+// ways, which are not resident at once, 29; 256 rows gate/up 2 x 4096 x 1536 in tiles of 128 13.9, of 64 22.7.
+int choose_shape(TileArgs& p, int sms) {
   double best = 0;
-  for (int bn = 32; bn <= 256; bn += 32) {
-    if (bn > 64 && bn - 32 >= p.a.M) break;  // wider than the rows there are
+  for (const int bn : {32, 64, 128, 256}) {
+    if (bn > 32 && bn / 2 >= p.a.M) break;  // wider than the rows there are
     const int64_t tiles = ((p.a.M + bn - 1) / bn) * p.f_tiles;
-    for (int split : {1, 2, 3, 4, 8}) {
-      if (split > 1 && (bn > 64 || tiles * split > sms || p.a.n_kb < 4 * split)) continue;
-      const double rounds = static_cast<double>((tiles * split + sms - 1) / sms);
-      const double stage = std::max(400.0, 2.0 * bn) + 0.4 * std::min(400.0, 2.0 * bn);
-      const double cost = rounds * ((p.a.n_kb + split - 1) / split) * stage + 10.0 * bn + (split > 1 ? 2500 : 0);
-      if (best == 0 || cost < best) {
-        best = cost;
+    for (const int split : {1, 2, 3, 4, 8}) {
+      int at_once = sms;
+      if (split > 1) {
+        if (bn > 64 || tiles * split > sms || p.a.n_kb < 4 * split) continue;
+        const auto kernel = tile_kernel<__nv_bfloat16, 64, false, true>;  // the others' resources are the same
+        LEMA_TRY(kernel_facts(reinterpret_cast<const void*>(kernel), Tile<64>::kSmemBytes, kTileThreads, split, &at_once));
+        if (at_once < 1) continue;
+      }
+      const double rounds = static_cast<double>((tiles + at_once - 1) / at_once);
+      const double stage = 0.36 + 0.0005 * std::max(0, bn - 128);
+      const double us = rounds * ((p.a.n_kb + split - 1) / split) * stage + 0.01 * bn + (split > 1 ? 1.5 : 0);
+      if (best == 0 || us < best) {
+        best = us;
         p.bn = bn;
         p.split = split;
         p.n_tiles = tiles;
       }
     }
   }
+  return LEMA_OK;
 }
 
 int run_tile(const Args& a, int dtype, bool gated, uint32_t* status, cudaStream_t stream) {
@@ -600,7 +609,7 @@ int run_tile(const Args& a, int dtype, bool gated, uint32_t* status, cudaStream_
   p.wait_ns = wait_limit_ns();
   p.f_tiles = (a.n_rb + kTileBlocks - 1) / kTileBlocks;
   p.pairs = a.N % 2 == 0 && a.ldy % 2 == 0 && aligned(a.y, 4) && (a.r == nullptr || (a.ldr % 2 == 0 && aligned(a.r, 4)));
-  choose_shape(p, dev->sms);
+  LEMA_TRY(choose_shape(p, dev->sms));
   CUtensorMap map;
   if (!encode_kmajor(enc, &map, a.x, a.M, a.K, a.ldx, p.bn,
                      dtype == LEMA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16))
