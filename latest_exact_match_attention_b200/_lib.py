@@ -157,8 +157,10 @@ def status_message(s: int, what: str) -> str:
 
 
 def stream_handle(device: torch.device | None = None) -> int:
-    """The raw cudaStream_t of torch's current stream on `device`."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """The raw cudaStream_t of torch's current stream on `device` (without the Stream object that
+    torch.cuda.current_stream makes: 0.1 instead of 2.3 us of host time a call)."""
+    idx = None if device is None else device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

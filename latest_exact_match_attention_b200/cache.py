@@ -46,6 +46,8 @@ _CARRIER = {torch.float32: torch.float32, torch.float16: torch.float16,
 _NP_TO_TORCH = {np.dtype(np.float32): torch.float32, np.dtype(np.float16): torch.float16,
                 np.dtype(np.uint16): torch.bfloat16}   # uint16 = the reference's bf16 carrier
 
+_ROWS_IN_ORDER = (0, 0, 0, 0, 0, 0, 0)   # lema_store_exchange_quant: item i's rows at i * d_v elements
+
 FULL_MESSAGE = ("hash table full: the store is presized and never grows -- provision more "
                 "capacity")
 
@@ -135,11 +137,12 @@ class HashStore:
         (heads, v_sb, v_sh, v_st, o_sb, o_sh, o_st) (bytes) the value and output rows of
         partition b * heads + h, position t are read and written at those strides instead
         (lema_store_exchange_strided): values and out may then be any views of that layout."""
-        qcodes, kcodes = qcodes.reshape(-1), kcodes.reshape(-1)
         if qcodes.dtype != kcodes.dtype:
             kcodes = kcodes.to(qcodes.dtype)
         cb = code_bytes_of(qcodes)
         n = qcodes.numel()
+        if kcodes.numel() != n:
+            raise ValueError(f"{n} query codes, {kcodes.numel()} key codes")
         P = n // T if T else 0
         if g0 < 0 or g0 + P > self.groups:
             raise ValueError(f"groups [{g0}, {g0 + P}) outside the store's {self.groups}")
@@ -154,7 +157,7 @@ class HashStore:
         ws = self._workspace(n, T, cb)
         qcodes, kcodes = qcodes.contiguous(), kcodes.contiguous()
         if rows is None:
-            if values.dim() != 2 or out.dim() != 2 or not out.is_contiguous():
+            if not out.is_contiguous():
                 raise ValueError("values and out must be [n, d_v] (out contiguous), or pass rows=")
             values = values.contiguous()
             call("lema_store_exchange_seg", ptr(self.table), self.cap, self.vbytes, ptr(qcodes),
@@ -171,21 +174,24 @@ class HashStore:
 
     def _exchange_quant(self, qcodes, kcodes, values, out, n, T, g0, rows, phase, check):
         """lema_store_exchange_quant: `exchange` and `exchange_phase` on quantised rows."""
-        codes = kcodes if qcodes is None else qcodes
-        for t in (values, out):
-            if t is not None and t.dtype != self.dtype:
-                raise ValueError(f"the store quantises {self.dtype} rows, got {t.dtype}")
+        dtype = self.dtype
+        if (values is not None and values.dtype != dtype) or (out is not None and out.dtype != dtype):
+            raise ValueError(f"the store quantises {dtype} rows, got {(out if values is None else values).dtype}")
         if rows is None:
-            if any(t is not None and t.dim() != 2 for t in (values, out)) or (out is not None and not out.is_contiguous()):
+            if out is not None and not out.is_contiguous():
                 raise ValueError("values and out must be [n, d_v] (out contiguous), or pass rows=")
-            values = None if values is None else values.contiguous()
-            rows = (0, 0, 0, 0, 0, 0, 0)
-        cb = code_bytes_of(codes)
-        ws = self._workspace(n, T, cb)
-        qcodes, kcodes = (None if c is None else c.contiguous() for c in (qcodes, kcodes))
-        args = ("lema_store_exchange_quant", ptr(self.table), self.cap, ROW_FORMATS[self.quant],
-                DTYPE_TAG[self.dtype], self.d_v, ptr(qcodes), ptr(kcodes), cb, ptr(values), ptr(out), n, T, g0,
-                ptr(self.counts) + 8 * g0, ptr(self.status), ptr(ws), 0 if ws is None else ws.numel(),
+            if values is not None and not values.is_contiguous():
+                values = values.contiguous()
+            rows = _ROWS_IN_ORDER
+        cb = code_bytes_of(kcodes if qcodes is None else qcodes)
+        if qcodes is not None and not qcodes.is_contiguous():
+            qcodes = qcodes.contiguous()
+        if kcodes is not None and not kcodes.is_contiguous():
+            kcodes = kcodes.contiguous()
+        ws = self._workspace(n, T, cb) if T > 1 else None
+        args = ("lema_store_exchange_quant", self.table.data_ptr(), self.cap, ROW_FORMATS[self.quant],
+                DTYPE_TAG[dtype], self.d_v, ptr(qcodes), ptr(kcodes), cb, ptr(values), ptr(out), n, T, g0,
+                self.counts.data_ptr() + 8 * g0, self.status.data_ptr(), ptr(ws), 0 if ws is None else ws.numel(),
                 self.seg_groups, self.seg_slots, *rows, phase, stream_handle(self.device))
         if self.device.index in (None, torch.cuda.current_device()):
             call(*args)
@@ -306,12 +312,9 @@ class LayerStore:
             rows = (H, v.stride(0) * es, v.stride(1) * es, v.stride(2) * es,
                     T * H * d_v * es, d_v * es, H * d_v * es)
             return Staging(qc.reshape(-1).contiguous(), kc.reshape(-1).contiguous(), v, out, T, rows)
-        vals = v.reshape(-1, d_v)
-        if not vals.is_contiguous():
-            vals = vals.contiguous()
-        out = (self.buffers.out(n, d_v, vals.device) if self.persistent_out
-               else torch.empty(n, d_v, dtype=vals.dtype, device=vals.device))
-        return Staging(qc.reshape(-1).contiguous(), kc.reshape(-1).contiguous(), vals, out, T)
+        vals = v if v.is_contiguous() else v.contiguous()
+        out = self.buffers.out(n, d_v, vals.device) if self.persistent_out else vals.new_empty(v.shape)
+        return Staging(qc.contiguous(), kc.contiguous(), vals, out, T)
 
     def host(self, s: Staging, check: bool = True):
         self.store.exchange(s.qc, s.kc, s.vals, s.out, s.T, self.g0, check=check, rows=s.rows)
@@ -319,7 +322,9 @@ class LayerStore:
     @staticmethod
     def retrieved(s: Staging, shape) -> torch.Tensor:
         """The retrieved rows as a [B, H, T, d_v] tensor (a view of the staging output)."""
-        return s.out.transpose(1, 2) if s.rows is not None else s.out.view(shape)
+        if s.rows is not None:
+            return s.out.transpose(1, 2)
+        return s.out if s.out.shape == shape else s.out.view(shape)
 
     @staticmethod
     def fetch(s: Staging, got: torch.Tensor):

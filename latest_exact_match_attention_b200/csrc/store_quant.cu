@@ -17,7 +17,12 @@
 // comes back as NaN (its scale is NaN): neither can be told by 8 bits of a shared scale.
 //
 // A group of G lanes serves one item (store.cu), lane j the values 8 j ... 8 j + 7, so d_v <= 8 G
-// and a row is one code word and one scale a lane. An in-chunk match (T > 1) reads the 16-bit row
+// and a row is one code word and one scale a lane. A decode step takes store.cu's groups (a round trip of
+// a long probe chain reads G headers); a prefill chunk's many items are bound by instructions and header
+// sectors instead and take the fewest lanes that hold a row, at least 4, and divide by multiplication.
+// 1024 partitions x 1024 positions of 24 values, load 0.5, overwriting:
+// resolve 138 -> 71 us, insert 125 -> 71; claiming new slots 312 -> 98 (one 16-byte compare-and-swap a claim
+// instead of lock, code, fence and state, and claims counted once a warp). An in-chunk match (T > 1) reads the 16-bit row
 // of its source and gives back the same numbers the store would: any chunking of a sequence gives
 // the same results.
 #include <cuda_bf16.h>
@@ -34,12 +39,24 @@ namespace k3 {
 
 constexpr int kMaxQuantDim = 256;  // 8 values a lane, at most 32 lanes an item
 
+// Division of n < 2^31 by a divisor known on the host: (mulhi(n, m) + n) >> s.
+struct Divisor {
+  uint32_t d, m, s;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by), s(0) {
+    while ((uint64_t(1) << s) < by) ++s;
+    m = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << s) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
 struct QArgs {
   Args a;          // a.vbytes: bytes of a held row; strides of v and out always set (a.heads >= 1)
   int d;           // values per row
   int chunks;      // of 8 values
   int cb;          // bytes per code word of codes, 4 or 8
   int v_vec, o_vec;  // whole chunks readable / writable as 16-byte words
+  Divisor by_t, by_heads;
 };
 
 template <int F> struct Format;  // F: LEMA_ROWS_*
@@ -219,26 +236,61 @@ __device__ __forceinline__ void store_frag(const QArgs& q, uint64_t s, const Fra
   const int pad = (static_cast<int>(q.a.vbytes) - codes) / 4 - groups;  // at most 3 words
   if (L.j < pad) scales[groups + L.j] = 0.f;
 }
+__device__ __forceinline__ const unsigned char* v_at(const QArgs& q, uint32_t p, uint32_t t) {
+  const uint32_t b = q.by_heads.quotient(p), h = p - b * q.by_heads.d;
+  return q.a.v + b * q.a.v_sb + h * q.a.v_sh + t * q.a.v_st;
+}
+__device__ __forceinline__ unsigned char* out_at(const QArgs& q, uint32_t p, uint32_t t) {
+  const uint32_t b = q.by_heads.quotient(p), h = p - b * q.by_heads.d;
+  return q.a.out + b * q.a.o_sb + h * q.a.o_sh + t * q.a.o_st;
+}
 template <typename T, int F, int G>
-__device__ __forceinline__ Frag<F> quantise_row(const QArgs& q, int64_t p, int64_t t, const Lane<G>& L) {
+__device__ __forceinline__ Frag<F> quantise_row(const QArgs& q, uint32_t p, uint32_t t, const Lane<G>& L) {
   float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = 0.f;
-  if (L.j < q.chunks) load8<T>(v_row<unsigned char>(q.a, p, t), L.j, q.d, q.v_vec, f);
+  if (L.j < q.chunks) load8<T>(v_at(q, p, t), L.j, q.d, q.v_vec, f);
   return quantise<F, G>(f, L);
 }
 template <typename T, int F, int G>
-__device__ __forceinline__ void emit_row(const QArgs& q, int64_t p, int64_t t, const Frag<F>& r, const Lane<G>& L) {
+__device__ __forceinline__ void emit_row(const QArgs& q, uint32_t p, uint32_t t, const Frag<F>& r, const Lane<G>& L) {
   if (L.j >= q.chunks) return;
   float f[8];
   values_of<F>(r, f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = saturate(f[i], Largest<T>::kV);
-  store8<T>(out_row<unsigned char>(q.a, p, t), L.j, q.d, q.o_vec, f);
+  store8<T>(out_at(q, p, t), L.j, q.d, q.o_vec, f);
 }
 
-__device__ __forceinline__ uint64_t code_at(const void* p, int64_t i, int cb) {
+__device__ __forceinline__ uint64_t code_at(const void* p, uint32_t i, int cb) {
   return cb == 4 ? static_cast<uint64_t>(static_cast<const uint32_t*>(p)[i]) : static_cast<const uint64_t*>(p)[i];
+}
+
+// (code, state) of slot s in one 16-byte access, as claim() writes them.
+__device__ __forceinline__ void read_slot(const Args& a, uint64_t s, uint64_t& code, uint64_t& state) {
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t"
+      "ld.relaxed.gpu.global.b128 h, [%2];\n\t"
+      "mov.b128 {%0, %1}, h;\n\t}"
+      : "=l"(code), "=l"(state)
+      : "l"(header(a, s))
+      : "memory");
+}
+// Empty -> (code, state) in one 16-byte compare-and-swap: a prober sees the slot empty or with its code, so the
+// slot needs no locked state and no release store behind the row. The row is read by later launches only: within
+// one launch nobody else looks for this (group, code).
+__device__ __forceinline__ int claim(uint64_t* hdr, uint64_t code, uint64_t state) {
+  uint64_t was_code, was_state;
+  asm volatile(
+      "{\n\t.reg .b128 e, n, o;\n\t"
+      "mov.b128 e, {%3, %3};\n\t"
+      "mov.b128 n, {%4, %5};\n\t"
+      "atom.relaxed.gpu.global.cas.b128 o, [%2], e, n;\n\t"
+      "mov.b128 {%0, %1}, o;\n\t}"
+      : "=l"(was_code), "=l"(was_state)
+      : "l"(hdr), "l"(kEmpty), "l"(code), "l"(state)
+      : "memory");
+  return (was_code | was_state) == 0;
 }
 
 // One item's lookup (want_q) and insert (want_k), their probes interleaved round trip by round
@@ -261,8 +313,8 @@ __device__ int probe(const QArgs& q, uint64_t g, uint64_t qcode, uint64_t kcode,
   if (want_q) spec = load_frag<F, G>(q, sq, L);  // a hit at home costs one round trip
   while (!qdone || kres == 2) {
     uint64_t qcd = 0, qst = 0, kcd = 0, kst = 0;
-    if (!qdone) read_header(a, wrap_add(sq, L.j, a.cap), qcd, qst);
-    if (kres == 2) read_header(a, wrap_add(sk, L.j, a.cap), kcd, kst);
+    if (!qdone) read_slot(a, wrap_add(sq, L.j, a.cap), qcd, qst);
+    if (kres == 2) read_slot(a, wrap_add(sk, L.j, a.cap), kcd, kst);
     if (!qdone) {
       const bool valid = tq + L.j < a.cap;  // no slot twice within one cycle of the table
       const unsigned hit = L.bits(__ballot_sync(L.gmask, valid && qst == tag && qcd == qcode));
@@ -291,15 +343,11 @@ __device__ int probe(const QArgs& q, uint64_t g, uint64_t qcode, uint64_t kcode,
           store_frag<F, G>(q, slot, mine, L);
           kres = 0;
         } else {
-          uint64_t* hdr = header(a, slot);
           int won = 0;
-          if (L.j == k) won = atomicCAS(reinterpret_cast<unsigned long long*>(hdr + 1), kEmpty, kLocked) == kEmpty;
+          if (L.j == k) won = claim(header(a, slot), kcode, tag);
           won = __shfl_sync(L.gmask, won, L.gbase + k);
           if (won) {
-            if (L.j == k) hdr[0] = kcode;
             store_frag<F, G>(q, slot, mine, L);
-            __syncwarp(L.gmask);
-            if (L.j == k) st_release(hdr + 1, tag);
             kres = 1;
           } else {
             sk = wrap_add(slot, 1, a.cap);
@@ -317,28 +365,35 @@ __device__ int probe(const QArgs& q, uint64_t g, uint64_t qcode, uint64_t kcode,
   return kres;
 }
 
-__device__ __forceinline__ void count_claim(const Args& a, int64_t p, int r) {
-  if (r < 0) {
-    raise_status(a.status, LEMA_STATUS_TABLE_FULL);
-  } else if (r > 0) {
-    atomicAdd(reinterpret_cast<unsigned long long*>(a.counts + p), 1ull);
-  }
+// r: probe's answer for partition p, in the first lane of each group (0 in the others). Whole warps call it: claims
+// of one partition are added once a warp.
+__device__ __forceinline__ void count_claims(const Args& a, uint32_t p, int r) {
+  if (r < 0) raise_status(a.status, LEMA_STATUS_TABLE_FULL);
+  const unsigned claims = __ballot_sync(kFullMask, r > 0);
+  if (claims == 0) return;
+  const int first = __ffs(claims) - 1;
+  const uint32_t of_first = __shfl_sync(kFullMask, p, first);  // by every lane, before the test that some would skip
+  const bool one = __all_sync(kFullMask, r <= 0 || p == of_first);
+  if (one ? (threadIdx.x & 31) == first : r > 0)
+    atomicAdd(reinterpret_cast<unsigned long long*>(a.counts + p), one ? static_cast<unsigned long long>(__popc(claims)) : 1ull);
 }
 
 // T == 1: item i is partition i; phase 3 looks up and inserts, 1 and 2 do one of the two.
 template <typename T, int F, int G>
 __global__ void __launch_bounds__(kThreads) quant_step(const QArgs q) {
   griddep_wait();  // launched as a dependent: the codes and values first
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / G;
-  if (i >= q.a.n) return;  // whole groups
+  const uint32_t i = blockIdx.x * (kThreads / G) + threadIdx.x / G;
   const Lane<G> L = group_lane<G>();
   const bool want_q = q.a.phase & 1, want_k = q.a.phase & 2;
-  const uint64_t qcode = want_q ? code_at(q.a.qc, i, q.cb) : 0, kcode = want_k ? code_at(q.a.kc, i, q.cb) : 0;
-  Frag<F> mine = zero_frag<F>(), got;
-  if (want_k) mine = quantise_row<T, F, G>(q, i, 0, L);
-  const int r = probe<F, G>(q, q.a.g0 + static_cast<uint64_t>(i), qcode, kcode, want_q, want_k, mine, got, L);
-  if (want_q) emit_row<T, F, G>(q, i, 0, got, L);
-  if (want_k && L.j == 0) count_claim(q.a, i, r);
+  int r = 0;
+  if (i < q.a.n) {  // whole groups
+    const uint64_t qcode = want_q ? code_at(q.a.qc, i, q.cb) : 0, kcode = want_k ? code_at(q.a.kc, i, q.cb) : 0;
+    Frag<F> mine = zero_frag<F>(), got;
+    if (want_k) mine = quantise_row<T, F, G>(q, i, 0, L);
+    r = probe<F, G>(q, q.a.g0 + i, qcode, kcode, want_q, want_k, mine, got, L);
+    if (want_q) emit_row<T, F, G>(q, i, 0, got, L);
+  }
+  if (want_k) count_claims(q.a, i, L.j == 0 ? r : 0);
 }
 
 // T > 1, after the matcher: a query with an in-chunk match gets the numbers its source row would
@@ -346,10 +401,10 @@ __global__ void __launch_bounds__(kThreads) quant_step(const QArgs q) {
 template <typename T, int F, int G>
 __global__ void __launch_bounds__(kThreads) quant_resolve(const QArgs q) {
   griddep_wait();
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / G;
+  const uint32_t i = blockIdx.x * (kThreads / G) + threadIdx.x / G;
   if (i >= q.a.n) return;
   const Lane<G> L = group_lane<G>();
-  const int64_t p = i / q.a.T;
+  const uint32_t p = q.by_t.quotient(i);
   const int32_t s = q.a.src[i];
   Frag<F> got;
   if (s >= 0) {
@@ -357,30 +412,33 @@ __global__ void __launch_bounds__(kThreads) quant_resolve(const QArgs q) {
   } else {
     probe<F, G>(q, q.a.g0 + static_cast<uint64_t>(p), code_at(q.a.qc, i, q.cb), 0, true, false, zero_frag<F>(), got, L);
   }
-  emit_row<T, F, G>(q, p, i - p * q.a.T, got, L);
+  emit_row<T, F, G>(q, p, i - p * q.by_t.d, got, L);
 }
 
 // T > 1: each partition's distinct key codes once, with the row of their last position.
 template <typename T, int F, int G>
 __global__ void __launch_bounds__(kThreads) quant_insert(const QArgs q) {
   griddep_wait();
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / G;
-  if (i >= q.a.n) return;
-  const int64_t p = i / q.a.T;
-  if (i - p * q.a.T >= q.a.lt_count[p]) return;  // whole groups
+  const uint32_t i = blockIdx.x * (kThreads / G) + threadIdx.x / G;
   const Lane<G> L = group_lane<G>();
-  const Frag<F> mine = quantise_row<T, F, G>(q, p, q.a.lt_pos[i], L);
-  Frag<F> got;
-  const int r = probe<F, G>(q, q.a.g0 + static_cast<uint64_t>(p), 0, code_at(q.a.lt_code, i, q.cb), false, true, mine, got, L);
-  if (L.j == 0) count_claim(q.a, p, r);
+  const uint32_t p = q.by_t.quotient(i);
+  int r = 0;
+  if (i < q.a.n && static_cast<int32_t>(i - p * q.by_t.d) < q.a.lt_count[p]) {  // whole groups
+    const Frag<F> mine = quantise_row<T, F, G>(q, p, q.a.lt_pos[i], L);
+    Frag<F> got;
+    r = probe<F, G>(q, q.a.g0 + p, 0, code_at(q.a.lt_code, i, q.cb), false, true, mine, got, L);
+  }
+  count_claims(q.a, p, L.j == 0 ? r : 0);
 }
 
 template <typename T, int F, int G>
 int run_quant(QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((q.a.n * G + kThreads - 1) / kThreads)), block(kThreads);
-  if (q.a.T == 1) {
-    LEMA_CUDA_TRY(launch_dependent(quant_step<T, F, G>, grid, block, 0, stream, q));
-    return LEMA_OK;
+  if constexpr (G >= 8) {
+    if (q.a.T == 1) {
+      LEMA_CUDA_TRY(launch_dependent(quant_step<T, F, G>, grid, block, 0, stream, q));
+      return LEMA_OK;
+    }
   }
   LEMA_TRY(chunk_match(q.a, ws, ws_bytes, q.cb, stream));
   LEMA_CUDA_TRY(launch_dependent(quant_resolve<T, F, G>, grid, block, 0, stream, q));
@@ -389,17 +447,20 @@ int run_quant(QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
 }
 
 template <typename T, int F>
-int run_lanes(int G, QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
+int run_lanes(QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  int G = q.a.T == 1 ? group_lanes(q.a.n) : 4;
+  while (G < q.chunks) G *= 2;
   if (G == 32) return run_quant<T, F, 32>(q, ws, ws_bytes, stream);
   if (G == 16) return run_quant<T, F, 16>(q, ws, ws_bytes, stream);
-  return run_quant<T, F, 8>(q, ws, ws_bytes, stream);
+  if (G == 8) return run_quant<T, F, 8>(q, ws, ws_bytes, stream);
+  return run_quant<T, F, 4>(q, ws, ws_bytes, stream);
 }
 
 template <typename T>
-int run_format(int format, int G, QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
-  if (format == LEMA_ROWS_INT8) return run_lanes<T, LEMA_ROWS_INT8>(G, q, ws, ws_bytes, stream);
-  if (format == LEMA_ROWS_FP8) return run_lanes<T, LEMA_ROWS_FP8>(G, q, ws, ws_bytes, stream);
-  return run_lanes<T, LEMA_ROWS_INT4>(G, q, ws, ws_bytes, stream);
+int run_format(int format, QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  if (format == LEMA_ROWS_INT8) return run_lanes<T, LEMA_ROWS_INT8>(q, ws, ws_bytes, stream);
+  if (format == LEMA_ROWS_FP8) return run_lanes<T, LEMA_ROWS_FP8>(q, ws, ws_bytes, stream);
+  return run_lanes<T, LEMA_ROWS_INT4>(q, ws, ws_bytes, stream);
 }
 
 }  // namespace k3
@@ -434,7 +495,7 @@ extern "C" int lema_store_exchange_quant(void* table, int64_t cap, int format, i
   if (code_bytes != 4 && code_bytes != 8) return fail(LEMA_ERR_INVALID_ARGUMENT, "code_bytes must be 4 or 8, got %d", code_bytes);
   if (cap < 1) return fail(LEMA_ERR_INVALID_ARGUMENT, "capacity must be >= 1 slot, got %lld", (long long)cap);
   if (n < 0 || T <= 0 || n % T != 0) return fail(LEMA_ERR_INVALID_ARGUMENT, "items must be partitions x T (n = %lld, T = %lld)", (long long)n, (long long)T);
-  if (n * 32 / k3::kThreads >= (int64_t(1) << 31) - 1) return fail(LEMA_ERR_INVALID_ARGUMENT, "too many items in one call (%lld)", (long long)n);
+  if (n >= (int64_t(1) << 31) || heads >= (int64_t(1) << 31)) return fail(LEMA_ERR_INVALID_ARGUMENT, "2^31 - 1 items in one call at most, got %lld", (long long)n);
   if (g0 < 0) return fail(LEMA_ERR_INVALID_ARGUMENT, "negative group offset");
   if (seg_groups < 0 || seg_slots < 0 || (seg_groups > 0) != (seg_slots > 0))
     return fail(LEMA_ERR_INVALID_ARGUMENT, "segments: groups and slots per segment both positive or both 0");
@@ -492,11 +553,10 @@ extern "C" int lema_store_exchange_quant(void* table, int64_t cap, int format, i
   q.cb = code_bytes;
   q.v_vec = aligned(values, 16) && (a.v_sb | a.v_sh | a.v_st) % 16 == 0;
   q.o_vec = aligned(out, 16) && (a.o_sb | a.o_sh | a.o_st) % 16 == 0;
-  // the lanes of store.cu for this many items, and at least one for each chunk of the row
-  int G = k3::group_lanes(n);
-  while (G < q.chunks) G *= 2;
+  q.by_t = k3::Divisor(static_cast<uint32_t>(T));
+  q.by_heads = k3::Divisor(static_cast<uint32_t>(a.heads));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == LEMA_F32) return k3::run_format<float>(format, G, q, workspace, workspace_bytes, s);
-  if (dtype == LEMA_BF16) return k3::run_format<__nv_bfloat16>(format, G, q, workspace, workspace_bytes, s);
-  return k3::run_format<__half>(format, G, q, workspace, workspace_bytes, s);
+  if (dtype == LEMA_F32) return k3::run_format<float>(format, q, workspace, workspace_bytes, s);
+  if (dtype == LEMA_BF16) return k3::run_format<__nv_bfloat16>(format, q, workspace, workspace_bytes, s);
+  return k3::run_format<__half>(format, q, workspace, workspace_bytes, s);
 }

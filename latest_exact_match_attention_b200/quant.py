@@ -144,38 +144,48 @@ class Int4Weight:
 
 
 def _product(name: str, x: torch.Tensor, w: Int4Weight, residual: torch.Tensor | None) -> torch.Tensor:
-    dev = require_cuda(x, w.packed, residual)
-    if x.dtype not in DTYPE_TAG:
+    # a decode step makes several of these calls a layer and its kernels take a few microseconds: the
+    # common case (rows side by side) stays short
+    packed, scales, k, n = w.packed, w.scales, w.k, w.n
+    dev = require_cuda(x, packed, residual)
+    tag = DTYPE_TAG.get(x.dtype)
+    if tag is None:
         raise LemaError(f"{name} takes fp32, bf16 or fp16 rows, got {x.dtype}")
-    k, n = w.k, w.n
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise LemaError(f"{name}: rows of {k} values wanted, got {tuple(x.shape)}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < k):
-        x2 = x2.contiguous()
-    M = x2.shape[0]
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise LemaError(f"{name}: rows of {k} values wanted, got {tuple(shape)}")
+    ldx = k
+    if not x.is_contiguous():
+        x = x if len(shape) == 2 else x.reshape(-1, k)
+        ldx = x.stride(0)
+        if x.stride(1) != 1 or (x.shape[0] > 1 and ldx < k):
+            x, ldx = x.contiguous(), k
+    M = x.numel() // k
+    y = x.new_empty((M, n)) if len(shape) == 2 else x.new_empty(shape[:-1] + (n,))
+    rp, ldr = None, n
     if residual is not None:
         if residual.shape != y.shape or residual.dtype != x.dtype:
             raise LemaError(f"{name}: the residual must be {x.dtype} {tuple(y.shape)}, got {residual.dtype} "
                             f"{tuple(residual.shape)}")
-        r2 = residual if residual.dim() == 2 else residual.reshape(-1, n)
-        if r2.stride(1) != 1 or (M > 1 and r2.stride(0) < n):
-            r2 = r2.contiguous()
+        if not residual.is_contiguous():
+            residual = residual if len(shape) == 2 else residual.reshape(-1, n)
+            ldr = residual.stride(0)
+            if residual.stride(1) != 1 or (M > 1 and ldr < n):
+                residual, ldr = residual.contiguous(), n
+        rp = residual.data_ptr()
     if M == 0:
         return y
-    tag = DTYPE_TAG[x.dtype]
-    args = (x2.data_ptr(), tag, M, k, x2.stride(0), w.packed.data_ptr(), w.scales.data_ptr(),
-            DTYPE_TAG[w.scales.dtype], w.group, n, 1 if w.gated else 0,
-            None if residual is None else r2.data_ptr(), n if residual is None else r2.stride(0), y.data_ptr(), n,
-            device_status(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
-    if dev.index == torch.cuda.current_device():
-        rc = lib().lema_int4_linear(*args)
+    idx = dev.index
+    args = (x.data_ptr(), tag, M, k, ldx, packed.data_ptr(), scales.data_ptr(), DTYPE_TAG[scales.dtype], w.group, n,
+            w.gated, rp, ldr, y.data_ptr(), n, device_status(dev).data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+    L = lib()
+    if idx == torch.cuda.current_device():
+        rc = L.lema_int4_linear(*args)
     else:
         with torch.cuda.device(dev):
-            rc = lib().lema_int4_linear(*args)
+            rc = L.lema_int4_linear(*args)
     if rc:
-        raise LemaError(f"{name} failed (code {rc}): {lib().lema_last_error().decode(errors='replace')}")
+        raise LemaError(f"{name} failed (code {rc}): {L.lema_last_error().decode(errors='replace')}")
     return y
 
 
@@ -203,6 +213,7 @@ class _Int4Module(nn.Module):
         self.n, self.k, self.group, self.gated = w.n, w.k, w.group, w.gated
         self.register_buffer("packed", w.packed)
         self.register_buffer("scales", w.scales)
+        self._weight = w
 
     def _apply(self, fn, recurse=True):
         # .to(dtype) casts floating buffers: the scales keep their own 16-bit type, uncast
@@ -214,7 +225,11 @@ class _Int4Module(nn.Module):
 
     @property
     def weight4(self) -> Int4Weight:
-        return Int4Weight(self.packed, self.scales, self.n, self.k, self.group, self.gated)
+        """The buffers as an Int4Weight (made anew when the module's buffers have been replaced)."""
+        w, packed, scales = self._weight, self.packed, self.scales
+        if w.packed is not packed or w.scales is not scales:
+            w = self._weight = Int4Weight(packed, scales, self.n, self.k, self.group, self.gated)
+        return w
 
     def extra_repr(self) -> str:
         return f"{self.k} -> {self.n}, 4 bits, group {self.group}"
