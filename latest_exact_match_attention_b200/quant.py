@@ -21,12 +21,13 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ._lib import DTYPE_TAG, LemaError, device_status, lib, require_cuda
+from ._lib import DTYPE_TAG, F32, LemaError, device_status, lib, require_cuda
 
 __all__ = ["Int4Weight", "Int4Linear", "Int4SwiGLU", "quantize_weight", "int4_linear", "int4_swiglu",
            "ROW_FORMATS", "row_bytes", "quantize_rows", "dequantize_rows"]
 
 GROUPS = (32, 64, 128)
+MANY_ROWS = 32      # more 16-bit rows go to the tcgen05 kernel of csrc/int4_tile.cu
 
 # ------------------------------------------------------------------ 4-bit weights
 
@@ -161,6 +162,12 @@ def _product(name: str, x: torch.Tensor, w: Int4Weight, residual: torch.Tensor |
         if x.stride(1) != 1 or (x.shape[0] > 1 and ldx < k):
             x, ldx = x.contiguous(), k
     M = x.numel() // k
+    if M > MANY_ROWS and tag != F32 and k >= 64 and ((ldx | x.data_ptr() >> 1) & 7):
+        # rows that the many-rows kernel cannot load in 16-byte pieces: an aligned copy of them
+        ldx = -(-k // 8) * 8
+        rows = x.new_empty((M, ldx))
+        rows[:, :k].copy_(x if x.dim() == 2 else x.view(M, k))
+        x = rows
     y = x.new_empty((M, n)) if len(shape) == 2 else x.new_empty(shape[:-1] + (n,))
     rp, ldr = None, n
     if residual is not None:

@@ -405,3 +405,19 @@ def test_graph_decoding_with_both_quantised(cuda, fmt, split, monkeypatch):
     assert a == b
     if fmt is not None:
         assert caches[0].nbytes() < m.new_cache("hbm", max_cache_len=64, batch=4).nbytes()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_unaligned_rows_take_the_many_rows_kernel(cuda, dtype):
+    """Odd widths and offsets are copied into aligned rows: the same numbers as from aligned rows of the same values."""
+    M, K, N = 90, 150, 64
+    c, s = weight(N, K, 64, dtype, 9, cuda)
+    w = Int4Weight.pack(c, s, 64)
+    room = torch.randn(M + 1, 160, device=cuda).to(dtype)
+    want = quant.int4_linear(room[:M, :K], w)                       # 16-byte aligned rows
+    assert torch.equal(quant.int4_linear(room[:M, :K].contiguous(), w), want)            # rows of 300 bytes
+    flat = torch.empty(M * 160 + 1, dtype=dtype, device=cuda)[1:]
+    flat.view(M, 160).copy_(room[:M])
+    assert torch.equal(quant.int4_linear(flat.view(M, 160)[:, :K], w), want)             # off by one element
+    assert torch.equal(quant.int4_linear(room[:M, :K].reshape(2, M // 2, K), w), want.view(2, M // 2, N))
+    assert torch.equal(quant.int4_linear(room[:M, :K].reshape(M // 2, 2, K).transpose(0, 1), w), want.view(M // 2, 2, N).transpose(0, 1))
