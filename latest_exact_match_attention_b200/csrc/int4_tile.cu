@@ -7,9 +7,11 @@
 //               accumulators; tcgen05.commit frees the stage;
 //   warps 2-5   epilogue: a lane holds one feature, a TMEM column one token; adds the residual or applies
 //               the activation (a gate and its up feature are 8 lanes apart) and rounds once;
-//   warps 6-21  dequantisation, four sets of 4 warps that take the stages in turn: each warp turns two blocks
-//               of 16 features x 64 inputs a stage into 16-bit floats and writes them where the MMA's A
-//               operand expects them (the same swizzle).
+//   the others  dequantisation, four sets of 2 or 4 warps that take the stages in turn: each warp turns four or
+//               two blocks of 16 features x 64 inputs a stage into 16-bit floats and writes them where the MMA's
+//               A operand expects them (the same swizzle). About 150 instructions a block of 1024 weights are
+//               what bounds the kernel: 0.36 us a stage in narrow tiles, 0.42 in tiles of 256 tokens, where the
+//               tensor cores alone would take 0.29.
 // Here a weight is rounded: s * q (8 + 4 significant bits, or 11 + 4) is rounded once to the rows' 16-bit
 // type, since the tensor core multiplies one type and a tile cannot scale its sums by groups without
 // reading the accumulator back every 32 to 128 inputs. That is half a step a weight, the rounding that a
@@ -30,16 +32,21 @@ using namespace tc;
 constexpr int kTileRows = 128;                    // weight rows a tile
 constexpr int kABytes = kTileRows * kBK * 2;      // 16 KiB
 constexpr int kTileBlocks = kTileRows / 16;       // block rows a tile
-constexpr int kSets = 4;                          // sets of dequantising warps; set i fills stages i, i + kSets, ...
-constexpr int kSetWarps = 4;
-constexpr int kMine = kTileBlocks / kSetWarps;    // block rows a warp
-constexpr int kTileThreads = 32 * (6 + kSets * kSetWarps);
+// Sets of dequantising warps; set i fills stages i, i + kSets, ... (no more sets than stages: a set may not wait for
+// the phase after the one that a stage is in).
+constexpr int kSets = 4;
 
 // Room for tiles of up to BN tokens. Clusters that split K (BN = 64 only) add the sums they receive.
 template <int BN>
 struct Tile {
   static constexpr int kStageBytes = kABytes + BN * kBK * 2;
   static constexpr int kStages = BN == 64 ? 8 : 4;
+  // narrow tiles are bound by how long a block takes, wide ones by the instructions for all of them: half the warps
+  // with twice the blocks each spend fewer on waiting and addresses (8192 rows gate/up 2 x 4096 x 1536: 166 -> 160 us;
+  // 64 rows 1536 x 4096 in narrow tiles: 9.0 -> 9.9)
+  static constexpr int kSetWarps = BN == 64 ? 4 : 2;
+  static constexpr int kMine = kTileBlocks / kSetWarps;  // block rows a warp
+  static constexpr int kThreads = 32 * (6 + kSets * kSetWarps);
   static constexpr uint32_t kTmemCols = 2 * BN;
   static constexpr int kUnitBytes = 8 * kTileRows * 4;  // 8 tokens of a tile's sums
   static constexpr int kRecvBytes = BN == 64 ? 7 * kUnitBytes : 0;
@@ -207,9 +214,9 @@ __device__ __forceinline__ void finish(const TileArgs& p, int row, int64_t m, co
 }
 
 template <typename T, int BN, bool kGated, bool kSame>
-__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_x, const TileArgs p) {
+__global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_x, const TileArgs p) {
   using TL = Tile<BN>;
-  constexpr int kStages = TL::kStages, kStageBytes = TL::kStageBytes;
+  constexpr int kStages = TL::kStages, kStageBytes = TL::kStageBytes, kSetWarps = TL::kSetWarps, kMine = TL::kMine;
   // instruction descriptor (tcgen05.mma kind::f16): fp32 accumulator, A and B of type T (0 fp16, 1 bf16), both
   // K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
   constexpr uint32_t kType = Pair<T>::kBf16;
@@ -534,7 +541,7 @@ int launch_tile(const CUtensorMap& map, const TileArgs& p, int grid, cudaStream_
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>(p.split), static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kTileThreads);
+  cfg.blockDim = dim3(Tile<BN>::kThreads);
   cfg.dynamicSmemBytes = Tile<BN>::kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -581,7 +588,7 @@ int choose_shape(TileArgs& p, int sms) {
       if (split > 1) {
         if (bn > 64 || tiles * split > sms || p.a.n_kb < 4 * split) continue;
         const auto kernel = tile_kernel<__nv_bfloat16, 64, false, true>;  // the others' resources are the same
-        LEMA_TRY(kernel_facts(reinterpret_cast<const void*>(kernel), Tile<64>::kSmemBytes, kTileThreads, split, &at_once));
+        LEMA_TRY(kernel_facts(reinterpret_cast<const void*>(kernel), Tile<64>::kSmemBytes, Tile<64>::kThreads, split, &at_once));
         if (at_once < 1) continue;
       }
       const double rounds = static_cast<double>((tiles + at_once - 1) / at_once);
