@@ -59,8 +59,11 @@ __device__ __forceinline__ Vec* out_row(const Args& a, int64_t p, int64_t t) {
 // when the table is segmented, onto the group's segment. Probing continues across segment
 // ends and wraps at cap either way, so capacity and fullness are those of one shared table;
 // segmenting only keeps one layer's exchange (its groups) inside a slice of the table.
+__device__ __forceinline__ uint64_t home_hash(uint64_t code, uint64_t group) {
+  return fmix64(code ^ fmix64(group ^ 0x5851F42D4C957F2Dull));
+}
 __device__ __forceinline__ uint64_t home(uint64_t code, uint64_t group, const Args& a) {
-  const uint64_t h = fmix64(code ^ fmix64(group ^ 0x5851F42D4C957F2Dull));
+  const uint64_t h = home_hash(code, group);
   if (a.seg_groups == 0) return __umul64hi(h, a.cap);
   return (group / a.seg_groups) * a.seg_slots + __umul64hi(h, a.seg_slots);
 }

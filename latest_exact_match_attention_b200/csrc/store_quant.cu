@@ -31,6 +31,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "store.cuh"
 
@@ -57,6 +58,7 @@ struct QArgs {
   int cb;          // bytes per code word of codes, 4 or 8
   int v_vec, o_vec;  // whole chunks readable / writable as 16-byte words
   Divisor by_t, by_heads;
+  uint64_t home_base, home_span;  // where the call's groups have their home slots, if in one segment (span > 0)
 };
 
 template <int F> struct Format;  // F: LEMA_ROWS_*
@@ -257,8 +259,11 @@ __device__ __forceinline__ void emit_row(const QArgs& q, uint32_t p, uint32_t t,
   if (L.j >= q.chunks) return;
   float f[8];
   values_of<F>(r, f);
+  // (an integer code's s * code is within a rounding of fp32 of the row's largest value: 16-bit types round it back)
+  if constexpr (F == LEMA_ROWS_FP8 || sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = saturate(f[i], Largest<T>::kV);
+    for (int i = 0; i < 8; ++i) f[i] = saturate(f[i], Largest<T>::kV);
+  }
   store8<T>(out_at(q, p, t), L.j, q.d, q.o_vec, f);
 }
 
@@ -266,6 +271,11 @@ __device__ __forceinline__ uint64_t code_at(const void* p, uint32_t i, int cb) {
   return cb == 4 ? static_cast<uint64_t>(static_cast<const uint32_t*>(p)[i]) : static_cast<const uint64_t*>(p)[i];
 }
 
+// home() without its division where all groups of the call share a segment (a layer's call does).
+__device__ __forceinline__ uint64_t home_of(const QArgs& q, uint64_t code, uint64_t group) {
+  if (q.home_span == 0) return home(code, group, q.a);
+  return q.home_base + __umul64hi(home_hash(code, group), q.home_span);
+}
 // (code, state) of slot s in one 16-byte access, as claim() writes them.
 __device__ __forceinline__ void read_slot(const Args& a, uint64_t s, uint64_t& code, uint64_t& state) {
   asm volatile(
@@ -304,7 +314,7 @@ __device__ int probe(const QArgs& q, uint64_t g, uint64_t qcode, uint64_t kcode,
                      const Frag<F>& mine, Frag<F>& got, const Lane<G>& L) {
   const Args& a = q.a;
   const uint64_t tag = g + 2;
-  uint64_t sq = want_q ? home(qcode, g, a) : 0, sk = want_k ? home(kcode, g, a) : 0;
+  uint64_t sq = want_q ? home_of(q, qcode, g) : 0, sk = want_k ? home_of(q, kcode, g) : 0;
   uint64_t tq = 0, tk = 0;
   bool qdone = !want_q;
   int kres = want_k ? 2 : 0;  // 2: probing
@@ -448,7 +458,10 @@ int run_quant(QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
 
 template <typename T, int F>
 int run_lanes(QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  // a decode step: store.cu's lanes, but 8 from 8192 items on (int8, 16384 items, load 0.65: 11.4 us with 8 lanes,
+  // 13.2 with 16, 18.0 with 32; 1024 items: 5.9, 4.4, 3.6)
   int G = q.a.T == 1 ? group_lanes(q.a.n) : 4;
+  if (G == kMidG && q.a.n > kMidMaxItems / 2 && std::getenv("LEMA_K3_GROUP") == nullptr) G = kG;
   while (G < q.chunks) G *= 2;
   if (G == 32) return run_quant<T, F, 32>(q, ws, ws_bytes, stream);
   if (G == 16) return run_quant<T, F, 16>(q, ws, ws_bytes, stream);
@@ -555,6 +568,12 @@ extern "C" int lema_store_exchange_quant(void* table, int64_t cap, int format, i
   q.o_vec = aligned(out, 16) && (a.o_sb | a.o_sh | a.o_st) % 16 == 0;
   q.by_t = k3::Divisor(static_cast<uint32_t>(T));
   q.by_heads = k3::Divisor(static_cast<uint32_t>(a.heads));
+  if (seg_groups == 0) {
+    q.home_span = a.cap;
+  } else if (g0 / seg_groups == (g0 + n / T - 1) / seg_groups) {
+    q.home_base = static_cast<uint64_t>(g0 / seg_groups * seg_slots);
+    q.home_span = a.seg_slots;
+  }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == LEMA_F32) return k3::run_format<float>(format, q, workspace, workspace_bytes, s);
   if (dtype == LEMA_BF16) return k3::run_format<__nv_bfloat16>(format, q, workspace, workspace_bytes, s);
