@@ -96,6 +96,7 @@ class HashStore:
         self.counts = torch.zeros(groups, dtype=torch.int64, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._ws = None
+        self._ws_held = []     # workspaces that captured graphs still use
         # segments > 1: each run of groups/segments groups (a layer, for LemaCache) has its
         # home slots in its own 1/segments of the table; results are the same either way
         segments = max(1, min(int(segments), groups, self.cap))
@@ -126,6 +127,8 @@ class HashStore:
                 raise LemaError("store workspace must be reserved before graph capture "
                                 "(HashStore.reserve)")
             self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        if torch.cuda.is_current_stream_capturing() and not any(self._ws is w for w in self._ws_held):
+            self._ws_held.append(self._ws)      # a replay uses it even after a larger call replaced it
         return self._ws
 
     def exchange(self, qcodes: torch.Tensor, kcodes: torch.Tensor, values: torch.Tensor,

@@ -31,7 +31,7 @@ from torch import nn
 from . import _lib
 from ._lib import DTYPE_TAG, call, check_status, device_status, ptr, stream_handle
 from .attention import pack_codes, prefill_match, proj_codes
-from .quant import Int4Linear, Int4SwiGLU
+from .quant import Int4Linear, Int4Module, Int4SwiGLU
 
 ATTN_KINDS = ("lema",)
 
@@ -358,6 +358,8 @@ class Transformer(nn.Module):
         an exact match needs every sign of a code, and rounding their weights flips signs.
         The model's parameters (and its caches' dtype) keep theirs; state dicts of a quantised model
         load into a model quantised with the same group."""
+        if any(isinstance(m, Int4Module) for m in self.modules()):
+            raise ValueError("the model's weights are quantised already")
         for b in self.blocks:
             b.attn.v_proj = Int4Linear.from_linear(b.attn.v_proj, group)
             b.attn.o_proj = Int4Linear.from_linear(b.attn.o_proj, group)
@@ -366,6 +368,11 @@ class Transformer(nn.Module):
         return self
 
     def n_params(self, embedding: bool = True) -> int:
-        """Parameter count; embedding=False leaves out the token embedding and the head."""
-        skip = set() if embedding else {id(self.tok_emb.weight), id(self.lm_head.weight)}
-        return sum(p.numel() for p in self.parameters() if id(p) not in skip)
+        """Parameter count (4-bit weights counted as weights); embedding=False leaves out the token
+        embedding and the head."""
+        n = sum(p.numel() for p in self.parameters())
+        n += sum(m.n_weights() for m in self.modules() if isinstance(m, Int4Module))
+        if embedding:
+            return n
+        head = self.lm_head
+        return n - self.tok_emb.weight.numel() - (head.n_weights() if isinstance(head, Int4Module) else head.weight.numel())

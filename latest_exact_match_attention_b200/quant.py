@@ -212,7 +212,7 @@ def int4_swiglu(x: torch.Tensor, w: Int4Weight) -> torch.Tensor:
     return _product("int4_swiglu", x, w, None)
 
 
-class _Int4Module(nn.Module):
+class Int4Module(nn.Module):
     """Holds an Int4Weight as buffers, so that it moves, saves and loads with the model."""
 
     def __init__(self, w: Int4Weight):
@@ -238,11 +238,14 @@ class _Int4Module(nn.Module):
             w = self._weight = Int4Weight(packed, scales, self.n, self.k, self.group, self.gated)
         return w
 
+    def n_weights(self) -> int:
+        return self.n * self.k * (2 if self.gated else 1)
+
     def extra_repr(self) -> str:
         return f"{self.k} -> {self.n}, 4 bits, group {self.group}"
 
 
-class Int4Linear(_Int4Module):
+class Int4Linear(Int4Module):
     """nn.Linear without bias, its weight in 4 bits."""
 
     @classmethod
@@ -261,7 +264,7 @@ class Int4SwiGLU(nn.Module):
 
     def __init__(self, gate_up: Int4Weight, down: Int4Weight):
         super().__init__()
-        self.gate_up = _Int4Module(gate_up)
+        self.gate_up = Int4Module(gate_up)
         self.down = Int4Linear(down)
 
     @classmethod

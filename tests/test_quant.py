@@ -182,3 +182,24 @@ def test_modules_keep_their_scales_and_load(tmp_path):
     assert torch.equal(m2.blocks[1].mlp.gate_up.packed, m.blocks[1].mlp.gate_up.packed)
     with pytest.raises(ValueError, match="bias"):
         quant.Int4Linear.from_linear(torch.nn.Linear(64, 16))
+
+
+def test_a_quantised_model_counts_copies_and_is_quantised_once():
+    import copy
+
+    from latest_exact_match_attention_b200.model import ModelConfig, Transformer
+    cfg = ModelConfig(vocab_size=128, depth=2, dim=64, num_heads=4, d_qk=32, d_v=16, dim_ff=128)
+    m = Transformer(cfg)
+    whole, body = m.n_params(), m.n_params(embedding=False)
+    m.quantize_weights_(group=64)
+    assert (m.n_params(), m.n_params(embedding=False)) == (whole, body)
+    with pytest.raises(ValueError, match="already"):
+        m.quantize_weights_()
+    w = m.lm_head.weight4
+    assert m.lm_head.weight4 is w
+    c = copy.deepcopy(m)
+    assert c.lm_head.weight4.packed is c.lm_head.packed and c.lm_head.packed is not m.lm_head.packed
+    m.lm_head.packed = m.lm_head.packed.clone()          # a replaced buffer is the weight from then on
+    assert m.lm_head.weight4.packed is m.lm_head.packed
+    with pytest.raises(ValueError, match="group"):
+        Transformer(cfg).quantize_weights_(group=48)

@@ -421,3 +421,90 @@ def test_unaligned_rows_take_the_many_rows_kernel(cuda, dtype):
     assert torch.equal(quant.int4_linear(flat.view(M, 160)[:, :K], w), want)             # off by one element
     assert torch.equal(quant.int4_linear(room[:M, :K].reshape(2, M // 2, K), w), want.view(2, M // 2, N))
     assert torch.equal(quant.int4_linear(room[:M, :K].reshape(M // 2, 2, K).transpose(0, 1), w), want.view(M // 2, 2, N).transpose(0, 1))
+
+
+@pytest.mark.parametrize("dtype,scale", [(BF16, F16), (F16, BF16), (F32, F16)])
+@pytest.mark.parametrize("M", [1, 12, 30, 100, 300])
+def test_scales_of_another_type_than_the_rows(cuda, M, dtype, scale):
+    N, K = 72, 320
+    c, s = weight(N, K, 64, scale, M, cuda)
+    assert s.dtype == scale
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(dtype).to(cuda)
+    got = quant.int4_linear(x, Int4Weight.pack(c, s, 64))
+    w = dense64(c, s, 64)
+    ref = x.double() @ w.t()
+    bound = sum_bound(x, w, dtype) * (1 + half_step(dtype)) + half_step(dtype) * ref.abs() + 2.0 ** -24 * (ref.abs() + 1)
+    assert bool(((got.double() - ref).abs() <= bound).all())
+    gu = quant.int4_swiglu(x, Int4Weight.pack_gate_up(c, s, c, s, 64))
+    assert bool(gu.isfinite().all()) and gu.shape == (M, N)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("K", [40, 64, 72, 96, 104, 136, 160, 200, 296])
+@pytest.mark.parametrize("M", [7, 33, 140])
+def test_every_tail_of_k(cuda, M, K, group):
+    """K ends inside a block, inside a half block and inside a scale group, in both kernels."""
+    N = 40
+    c, s = weight(N, K, group, BF16, K, cuda)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(K)).to(BF16).to(cuda)
+    got = quant.int4_linear(x, Int4Weight.pack(c, s, group))
+    w = dense64(c, s, group)
+    ref = x.double() @ w.t()
+    bound = sum_bound(x, w, BF16) * (1 + half_step(BF16)) + half_step(BF16) * ref.abs() + 2.0 ** -24 * (ref.abs() + 1)
+    assert bool(((got.double() - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(4096, 1024, 8192), (64, 128, 65536)])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_exact(cuda, monkeypatch, M, N, K):
+    """Waits bounded to 1 ns run out (tiles alone, and tiles whose K a cluster splits): the status word says so, nothing
+    hangs, and the next call with the usual bound gives the bits of the first. A wait is given up after eight tries,
+    which the hardware may each suspend for about a microsecond: an accumulator here takes 128 stages, over 40 us."""
+    c, s = weight(N, K, 128, BF16, 0, cuda)
+    w = Int4Weight.pack(c, s, 128)
+    x = torch.randn(M, K, device=cuda).to(BF16)
+    want = quant.int4_linear(x, w)
+    check_status(cuda)
+    monkeypatch.setenv("LEMA_WAIT_NS", "1")
+    quant.int4_linear(x, w)
+    torch.cuda.synchronize()
+    with pytest.raises(LemaError, match="ran out"):
+        check_status(cuda, "int4_linear")
+    monkeypatch.delenv("LEMA_WAIT_NS")
+    assert torch.equal(quant.int4_linear(x, w), want)
+    check_status(cuda)
+
+
+def test_a_captured_chunk_keeps_its_workspace(cuda):
+    """A graph of a prefill chunk still replays after a larger eager call replaced the store's workspace."""
+    P, T, d = 4, 64, 24
+    rng = np.random.default_rng(3)
+    st = HashStore(d, groups=P, dtype=BF16, capacity=40000, device=cuda, quant="int8")
+    q, k, v = (t.to(cuda) for t in stream(rng, P, T, d, BF16, span=500))
+    out = torch.empty(P * T, d, dtype=BF16, device=cuda)
+    st.exchange(q, k, v, out, T, 0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st.exchange(q, k, v, out, T, 0, check=False)
+    want = torch.empty_like(out)
+    st.exchange(q, k, v, want, T, 0)
+    big = [t.to(cuda) for t in stream(rng, P, 40 * T, d, BF16, span=500)]
+    codes = [b + 1000 for b in big[:2]]                       # other codes: the graph's own entries stay
+    st.exchange(*codes, big[2], torch.empty(P * 40 * T, d, dtype=BF16, device=cuda), 40 * T, 0)
+    fill = [torch.randint(0, 255, (1 << 20,), dtype=torch.uint8, device=cuda) for _ in range(8)]
+    graph.replay()
+    st.check()
+    assert torch.equal(out, want) and len(fill) == 8
+
+
+def test_other_shapes_of_codes_and_rows_are_the_same_items(cuda):
+    B, H, d = 3, 4, 16
+    st = [HashStore(d, groups=B * H, dtype=BF16, capacity=1000, device=cuda, quant="int8") for _ in range(2)]
+    k = torch.arange(B * H, dtype=torch.int32, device=cuda) % 5
+    v = torch.randn(B * H, d, device=cuda).to(BF16)
+    out = [torch.empty(B * H, d, dtype=BF16, device=cuda), torch.empty(B, H, 1, d, dtype=BF16, device=cuda)]
+    for _ in range(2):
+        st[0].exchange(k, k, v, out[0], 1, 0)
+        st[1].exchange(k.view(B, H, 1), k.view(B, H, 1), v.view(B, H, 1, d), out[1], 1, 0)
+        assert torch.equal(out[0], out[1].view(B * H, d))
+    with pytest.raises(ValueError, match="key codes"):
+        st[0].exchange(k, k[:5], v, out[0], 1, 0)
