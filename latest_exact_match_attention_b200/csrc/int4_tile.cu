@@ -9,9 +9,13 @@
 //               the activation (a gate and its up feature are 8 lanes apart) and rounds once;
 //   the others  dequantisation, four sets of 2 or 4 warps that take the stages in turn: each warp turns four or
 //               two blocks of 16 features x 64 inputs a stage into 16-bit floats and writes them where the MMA's
-//               A operand expects them (the same swizzle). About 150 instructions a block of 1024 weights are
-//               what bounds the kernel: 0.36 us a stage in narrow tiles, 0.42 in tiles of 256 tokens, where the
-//               tensor cores alone would take 0.29.
+//               A operand expects them (the same swizzle). Its words and scales are loaded a stage of its own
+//               ahead. (Brought by TMA into a ring in shared memory instead they were 1 to 3% faster, and wrong
+//               unless a slot was given back only behind the proxy fence that follows the last use of its words.)
+// What bounds it, measured with parts left out: 8192 rows through 4096 x 4096 take 207 us, 6% less without the
+// subtraction and the product of every weight, 166 where the tensor cores wait for no weights at all; a stage takes
+// 0.36 us in narrow tiles (0.21 without dequantisation: four MMAs of 64 tokens, their issue and the ring's waits)
+// and 0.42 in tiles of 256 tokens.
 // Here a weight is rounded: s * q (8 + 4 significant bits, or 11 + 4) is rounded once to the rows' 16-bit
 // type, since the tensor core multiplies one type and a tile cannot scale its sums by groups without
 // reading the accumulator back every 32 to 128 inputs. That is half a step a weight, the rounding that a
@@ -32,8 +36,9 @@ using namespace tc;
 constexpr int kTileRows = 128;                    // weight rows a tile
 constexpr int kABytes = kTileRows * kBK * 2;      // 16 KiB
 constexpr int kTileBlocks = kTileRows / 16;       // block rows a tile
-// Sets of dequantising warps; set i fills stages i, i + kSets, ... (no more sets than stages: a set may not wait for
-// the phase after the one that a stage is in).
+// Sets of dequantising warps; set i fills stages i, i + kSets, ... Stages are a multiple of kSets, so that the phase
+// before the one that a set waits for is one that this set has seen: a parity cannot tell a phase from the one two
+// before it.
 constexpr int kSets = 4;
 
 // Room for tiles of up to BN tokens. Clusters that split K (BN = 64 only) add the sums they receive.

@@ -27,7 +27,7 @@ __all__ = ["Int4Weight", "Int4Linear", "Int4SwiGLU", "quantize_weight", "int4_li
            "ROW_FORMATS", "row_bytes", "quantize_rows", "dequantize_rows"]
 
 GROUPS = (32, 64, 128)
-MANY_ROWS = 32      # more 16-bit rows go to the tcgen05 kernel of csrc/int4_tile.cu
+COPY_ROWS = 128     # more unaligned 16-bit rows than this are worth a copy for the tcgen05 kernel
 
 # ------------------------------------------------------------------ 4-bit weights
 
@@ -162,8 +162,9 @@ def _product(name: str, x: torch.Tensor, w: Int4Weight, residual: torch.Tensor |
         if x.stride(1) != 1 or (x.shape[0] > 1 and ldx < k):
             x, ldx = x.contiguous(), k
     M = x.numel() // k
-    if M > MANY_ROWS and tag != F32 and k >= 64 and ((ldx | x.data_ptr() >> 1) & 7):
-        # rows that the many-rows kernel cannot load in 16-byte pieces: an aligned copy of them
+    if M > COPY_ROWS and tag != F32 and k >= 64 and ((ldx | x.data_ptr() >> 1) & 7):
+        # rows that the many-rows kernel cannot load in 16-byte pieces: an aligned copy of them (fewer take the
+        # few-rows kernel as they are: 37 rows of 1100 in 13 us, less than the host time of a copy)
         ldx = -(-k // 8) * 8
         rows = x.new_empty((M, ldx))
         rows[:, :k].copy_(x if x.dim() == 2 else x.view(M, k))

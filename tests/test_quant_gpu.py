@@ -410,7 +410,7 @@ def test_graph_decoding_with_both_quantised(cuda, fmt, split, monkeypatch):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_unaligned_rows_take_the_many_rows_kernel(cuda, dtype):
     """Odd widths and offsets are copied into aligned rows: the same numbers as from aligned rows of the same values."""
-    M, K, N = 90, 150, 64
+    M, K, N = 180, 150, 64
     c, s = weight(N, K, 64, dtype, 9, cuda)
     w = Int4Weight.pack(c, s, 64)
     room = torch.randn(M + 1, 160, device=cuda).to(dtype)
@@ -508,3 +508,22 @@ def test_other_shapes_of_codes_and_rows_are_the_same_items(cuda):
         assert torch.equal(out[0], out[1].view(B * H, d))
     with pytest.raises(ValueError, match="key codes"):
         st[0].exchange(k, k[:5], v, out[0], 1, 0)
+
+
+@pytest.mark.parametrize("M,N,K,group,gated", [(4096, 512, 1536, 128, True), (6000, 1536, 1024, 64, False), (3000, 1000, 1096, 32, False),
+                                               (512, 2048, 1536, 128, True), (200, 1536, 4096, 128, False), (40, 1536, 1536, 32, True)])
+def test_many_rows_give_the_same_bits_every_time(cuda, M, N, K, group, gated):
+    """Back to back, and behind passes that empty the caches: a missing wait anywhere in the ring shows as other bits."""
+    c, s = weight(N, K, group, BF16, M, cuda)
+    w = Int4Weight.pack_gate_up(c, s, c, s, group) if gated else Int4Weight.pack(c, s, group)
+    call = quant.int4_swiglu if gated else quant.int4_linear
+    x = torch.randn(M, K, device=cuda).to(BF16)
+    want = call(x, w).clone()
+    room = torch.empty(256 << 20, dtype=torch.uint8, device=cuda)
+    other = torch.zeros((), dtype=torch.long, device=cuda)
+    for i in range(60):
+        if i % 3 == 0:
+            room.fill_(i)
+        other += (call(x, w) != want).sum()
+    assert int(other) == 0
+    check_status(cuda)
