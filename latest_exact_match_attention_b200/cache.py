@@ -90,6 +90,7 @@ class HashStore:
             "cuda", torch.cuda.current_device())
         if self.device.type != "cuda":
             raise LemaError("the B200 store lives in device memory; device must be CUDA")
+        self._index = self.device.index
         self.stride = int(_lib.lib().lema_store_slot_bytes(self.vbytes))
         self.cap = max(16, int(capacity))
         self.table = torch.zeros((self.cap, self.stride), dtype=torch.uint8, device=self.device)
@@ -196,7 +197,7 @@ class HashStore:
                 DTYPE_TAG[dtype], self.d_v, ptr(qcodes), ptr(kcodes), cb, ptr(values), ptr(out), n, T, g0,
                 self.counts.data_ptr() + 8 * g0, self.status.data_ptr(), ptr(ws), 0 if ws is None else ws.numel(),
                 self.seg_groups, self.seg_slots, *rows, phase, stream_handle(self.device))
-        if self.device.index in (None, torch.cuda.current_device()):
+        if self._index is None or self._index == torch._C._cuda_getDevice():
             call(*args)
         else:
             with torch.cuda.device(self.device):
@@ -351,6 +352,17 @@ class LayerStore:
                  check: bool = True) -> torch.Tensor:
         """Look up every query, fold in every key: the values each query retrieves,
         `[B, H, T, d_v]` like `v`, zeros where nothing matched."""
+        st = self.store
+        if (st.quant is not None and v.dim() == 4 and v.shape[2] == 1 and self.buffers.codes_hook is None
+                and not self.persistent_out):
+            # a decode step on quantised rows: the same checks and one call, without the staging object
+            n = qc.numel()
+            if n != self.partitions or kc.numel() != n or kc.dtype != qc.dtype or v.numel() != n * st.d_v or v.shape[3] != st.d_v:
+                raise ValueError(f"a step's codes and values must be [B, H, 1] and [B, H, 1, {st.d_v}] of {self.partitions} "
+                                 f"partitions, got {tuple(qc.shape)}, {tuple(kc.shape)} and {tuple(v.shape)}")
+            out = v.new_empty(v.shape)
+            st._exchange_quant(qc, kc, v, out, n, 1, self.g0, None, 3, check and not torch.cuda.is_current_stream_capturing())
+            return out
         s = self.stage(qc, kc, v)
         self.host(s, check=check and not torch.cuda.is_current_stream_capturing())
         return self.retrieved(s, v.shape)

@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ._lib import DTYPE_TAG, F32, LemaError, device_status, lib, require_cuda
+from ._lib import DTYPE_TAG, F32, LemaError, _status_words, device_status, lib, require_cuda
 
 __all__ = ["Int4Weight", "Int4Linear", "Int4SwiGLU", "quantize_weight", "int4_linear", "int4_swiglu",
            "ROW_FORMATS", "row_bytes", "quantize_rows", "dequantize_rows"]
@@ -147,8 +147,10 @@ class Int4Weight:
 def _product(name: str, x: torch.Tensor, w: Int4Weight, residual: torch.Tensor | None) -> torch.Tensor:
     # a decode step makes several of these calls a layer and its kernels take a few microseconds: the
     # common case (rows side by side) stays short
-    packed, scales, k, n = w.packed, w.scales, w.k, w.n
-    dev = require_cuda(x, packed, residual)
+    packed, k, n = w.packed, w.k, w.n
+    dev = packed.device
+    if x.device != dev or not x.is_cuda or (residual is not None and residual.device != dev):
+        require_cuda(x, packed, residual)
     tag = DTYPE_TAG.get(x.dtype)
     if tag is None:
         raise LemaError(f"{name} takes fp32, bf16 or fp16 rows, got {x.dtype}")
@@ -183,11 +185,14 @@ def _product(name: str, x: torch.Tensor, w: Int4Weight, residual: torch.Tensor |
         rp = residual.data_ptr()
     if M == 0:
         return y
-    idx = dev.index
+    idx, scales = dev.index, w.scales
+    status = _status_words.get(idx)
+    if status is None:
+        status = device_status(dev)
     args = (x.data_ptr(), tag, M, k, ldx, packed.data_ptr(), scales.data_ptr(), DTYPE_TAG[scales.dtype], w.group, n,
-            w.gated, rp, ldr, y.data_ptr(), n, device_status(dev).data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+            w.gated, rp, ldr, y.data_ptr(), n, status.data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
     L = lib()
-    if idx == torch.cuda.current_device():
+    if idx == torch._C._cuda_getDevice():
         rc = L.lema_int4_linear(*args)
     else:
         with torch.cuda.device(dev):
