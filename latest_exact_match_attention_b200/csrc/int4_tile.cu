@@ -41,7 +41,7 @@ constexpr int kTileBlocks = kTileRows / 16;       // block rows a tile
 // before it.
 constexpr int kSets = 4;
 
-// Room for tiles of up to BN tokens. Clusters that split K (BN = 64 only) add the sums they receive.
+// Room for tiles of up to BN tokens.
 template <int BN>
 struct Tile {
   static constexpr int kStageBytes = kABytes + BN * kBK * 2;
@@ -54,8 +54,7 @@ struct Tile {
   static constexpr int kThreads = 32 * (6 + kSets * kSetWarps);
   static constexpr uint32_t kTmemCols = 2 * BN;
   static constexpr int kUnitBytes = 8 * kTileRows * 4;  // 8 tokens of a tile's sums
-  static constexpr int kRecvBytes = BN == 64 ? 7 * kUnitBytes : 0;
-  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kRecvBytes + 1024 /* alignment */ + 512 /* barriers */;
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + 1024 /* alignment */ + 512 /* barriers */;
 };
 
 struct TileArgs {
@@ -218,7 +217,7 @@ __device__ __forceinline__ void finish(const TileArgs& p, int row, int64_t m, co
   }
 }
 
-template <typename T, int BN, bool kGated, bool kSame>
+template <typename T, int BN, bool kGated, bool kSame, bool kSplit>
 __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_x, const TileArgs p) {
   using TL = Tile<BN>;
   constexpr int kStages = TL::kStages, kStageBytes = TL::kStageBytes, kSetWarps = TL::kSetWarps, kMine = TL::kMine;
@@ -231,8 +230,7 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
   const uint32_t raw = smem_addr(smem_raw);
   unsigned char* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
   const uint32_t sbase = smem_addr(smem);
-  const uint32_t recv = sbase + kStages * kStageBytes;  // sums of other CTAs of a split tile
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes + TL::kRecvBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
   // barriers: x full, weights full, empty [kStages each], acc_full[2], acc_empty[2], drain
   const uint32_t bar0 = smem_addr(bars);
   auto xfull_bar = [&](int s) { return bar0 + 8u * s; };
@@ -249,7 +247,7 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
   // this CTA's tiles, and its share of their K blocks
   // (grid: x the CTAs of a cluster, y the tiles; read as blockIdx and gridDim everywhere, which keeps the loops'
   // counters and the MMA's descriptors in uniform registers: copies of them cost 8% at 16384 rows)
-  const int split = BN == 64 ? p.split : 1, rank = BN == 64 ? static_cast<int>(blockIdx.x) : 0;
+  const int split = kSplit ? p.split : 1, rank = kSplit ? static_cast<int>(blockIdx.x) : 0;
   const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * a.n_kb / split);
   const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * a.n_kb / split);
   if (threadIdx.x == 0) {
@@ -277,7 +275,6 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
-  if (split > 1) cluster_arrive();  // answered before the first store into another CTA
   griddep_launch();
   griddep_wait();  // launched as a dependent: x and the residual are read only from here on
 
@@ -354,7 +351,7 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     int acc = 0;
     uint32_t aph = 0;
-    for (int64_t tile = blockIdx.y; split == 1 && tile < p.n_tiles; tile += gridDim.y) {
+    for (int64_t tile = blockIdx.y; !kSplit && tile < p.n_tiles; tile += gridDim.y) {
       if (!warp_wait(accf_bar(acc), aph, s_abort, p.status, p.wait_ns)) break;
       tc_fence_after();
       const int64_t m0 = (tile / p.f_tiles) * p.bn;
@@ -460,69 +457,73 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
   done:;
   }
 
-  if constexpr (BN == 64) {
-    if (split > 1) {
-      // One tile a cluster: CTA q of it finishes units u = q, q + split, ... of 8 tokens. Every CTA sends its sums
-      // of the others' units, all meet, and the sums are added in the order of the ranks.
-      const int64_t m0 = static_cast<int64_t>(blockIdx.y / p.f_tiles) * p.bn;
-      const int quarter = warp & 3, row_in = quarter * 32 + lane;
-      const int row = static_cast<int>(blockIdx.y % p.f_tiles) * kTileRows + row_in;
-      const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-      const bool live = warp >= 2 && warp < 6;
-      const int slots = (p.bn / 8 + split - 1) / split;  // units of one CTA
-      // where source q's sums of my unit k lie: [q or q - 1][k][two halves of 4 tokens][128 rows]
-      auto place = [&](int src, int dst, int k) {
-        return recv + static_cast<uint32_t>(((src < dst ? src : src - 1) * slots + k) * TL::kUnitBytes + row_in * 16);
-      };
-      bool ok = false;
-      cluster_wait();
-      if (live) {
-        ok = warp_wait(accf_bar(0), 0, s_abort, p.status, p.wait_ns);
-        tc_fence_after();
-        for (int u = 0; u < p.bn / 8; ++u) {
-          const int to = u % split;
-          if (to == rank || m0 + u * 8 >= a.M || !ok) continue;  // warp-uniform
-          uint32_t r[8];
-          tmem_load8(tmem_base + lane_base + static_cast<uint32_t>(u * 8), r);
-          const uint32_t at = place(rank, to, u / split);
+  if constexpr (kSplit) {
+    // One tile a cluster: CTA q of it finishes units u = q, q + split, ... of 8 tokens. When all CTAs' products are done,
+    // and with them the last read of any stage, every CTA sends its sums of the others' units over their stages; all
+    // meet again, and the sums are added in the order of the ranks.
+    const int64_t m0 = static_cast<int64_t>(blockIdx.y / p.f_tiles) * p.bn;
+    const int quarter = warp & 3, row_in = quarter * 32 + lane;
+    const int row = static_cast<int>(blockIdx.y % p.f_tiles) * kTileRows + row_in;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const bool live = warp >= 2 && warp < 6;
+    const int mine = (p.bn / 8 + split - 1) / split;  // units of one CTA
+    // where source q's sums of my unit k lie: [q or q - 1][k][two halves of 4 tokens][128 rows]; with at most 32 units
+    // and 8 CTAs that is 28 units of 4 KiB, less than the stages hold
+    auto place = [&](int src, int dst, int k) {
+      return sbase + static_cast<uint32_t>(((src < dst ? src : src - 1) * mine + k) * TL::kUnitBytes + row_in * 16);
+    };
+    bool ok = false;
+    if (live) {
+      ok = warp_wait(accf_bar(0), 0, s_abort, p.status, p.wait_ns);
+      tc_fence_after();
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (live && ok) {
+      for (int u = 0; u < p.bn / 8; ++u) {
+        const int to = u % split;
+        if (to == rank || m0 + u * 8 >= a.M) continue;  // warp-uniform
+        uint32_t r[8];
+        tmem_load8(tmem_base + lane_base + static_cast<uint32_t>(u * 8), r);
+        const uint32_t at = place(rank, to, u / split);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            store_remote(at + h * (TL::kUnitBytes / 2), to, __uint_as_float(r[4 * h]), __uint_as_float(r[4 * h + 1]),
-                         __uint_as_float(r[4 * h + 2]), __uint_as_float(r[4 * h + 3]));
-        }
+        for (int h = 0; h < 2; ++h)
+          store_remote(at + h * (TL::kUnitBytes / 2), to, __uint_as_float(r[4 * h]), __uint_as_float(r[4 * h + 1]),
+                       __uint_as_float(r[4 * h + 2]), __uint_as_float(r[4 * h + 3]));
       }
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();
-      if (live && ok) {
-        for (int k = 0; k < slots; ++k) {
-          const int u = k * split + rank;
-          if (u * 8 >= p.bn || m0 + u * 8 >= a.M) break;  // warp-uniform
-          uint32_t r[8];
-          tmem_load8(tmem_base + lane_base + static_cast<uint32_t>(u * 8), r);
-          float v[8];
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (live && ok) {
+      for (int k = 0; k < mine; ++k) {
+        const int u = k * split + rank;
+        if (u * 8 >= p.bn || m0 + u * 8 >= a.M) break;  // warp-uniform
+        uint32_t r[8];
+        tmem_load8(tmem_base + lane_base + static_cast<uint32_t>(u * 8), r);
+        float v[8];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) v[c] = 0.f;
-          for (int q = 0; q < split; ++q) {
-            if (q == rank) {
+        for (int c = 0; c < 8; ++c) v[c] = 0.f;
+        for (int q = 0; q < split; ++q) {
+          if (q == rank) {
 #pragma unroll
-              for (int c = 0; c < 8; ++c) v[c] += __uint_as_float(r[c]);
-              continue;
-            }
-            const uint32_t at = place(q, rank, k);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float f[4];
-              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                           : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
-                           : "r"(at + h * (TL::kUnitBytes / 2))
-                           : "memory");
-#pragma unroll
-              for (int c = 0; c < 4; ++c) v[4 * h + c] += f[c];
-            }
+            for (int c = 0; c < 8; ++c) v[c] += __uint_as_float(r[c]);
+            continue;
           }
-          finish<T, kGated, 8>(p, row, m0 + u * 8, v);
+          const uint32_t at = place(q, rank, k);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float f[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
+                         : "r"(at + h * (TL::kUnitBytes / 2))
+                         : "memory");
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[4 * h + c] += f[c];
+          }
         }
+        finish<T, kGated, 8>(p, row, m0 + u * 8, v);
       }
     }
   }
@@ -539,9 +540,9 @@ bool tile_ok(const Args& a, int dtype) {
   return dtype != LEMA_F32 && a.K >= kBK && (a.ldx * 2) % 16 == 0 && aligned(a.x, 16);
 }
 
-template <typename T, int BN, bool kGated, bool kSame>
+template <typename T, int BN, bool kGated, bool kSame, bool kSplit>
 int launch_tile(const CUtensorMap& map, const TileArgs& p, int grid, cudaStream_t stream) {
-  const auto kernel = tile_kernel<T, BN, kGated, kSame>;
+  const auto kernel = tile_kernel<T, BN, kGated, kSame, kSplit>;
   LEMA_TRY(kernel_facts(reinterpret_cast<const void*>(kernel), Tile<BN>::kSmemBytes, 0, 0, nullptr));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
@@ -564,11 +565,17 @@ int launch_tile(const CUtensorMap& map, const TileArgs& p, int grid, cudaStream_
   return LEMA_OK;
 }
 
+template <typename T, int BN, bool kGated, bool kSame>
+int launch_split(const CUtensorMap& map, const TileArgs& p, int grid, cudaStream_t stream) {
+  if (p.split > 1) return launch_tile<T, BN, kGated, kSame, true>(map, p, grid, stream);
+  return launch_tile<T, BN, kGated, kSame, false>(map, p, grid, stream);
+}
+
 template <typename T, int BN>
 int launch_width(const CUtensorMap& map, const TileArgs& p, int grid, bool gated, cudaStream_t stream) {
   const bool same = p.a.scale_bf16 == Pair<T>::kBf16;
-  if (gated) return same ? launch_tile<T, BN, true, true>(map, p, grid, stream) : launch_tile<T, BN, true, false>(map, p, grid, stream);
-  return same ? launch_tile<T, BN, false, true>(map, p, grid, stream) : launch_tile<T, BN, false, false>(map, p, grid, stream);
+  if (gated) return same ? launch_split<T, BN, true, true>(map, p, grid, stream) : launch_split<T, BN, true, false>(map, p, grid, stream);
+  return same ? launch_split<T, BN, false, true>(map, p, grid, stream) : launch_split<T, BN, false, false>(map, p, grid, stream);
 }
 
 template <typename T>
@@ -580,25 +587,33 @@ int launch_type(const CUtensorMap& map, const TileArgs& p, int grid, bool gated,
 
 // The tile width and the split of K with the least estimated time (us): rounds of tiles over the SMs, or of
 // clusters over what can be resident at once, each of n_kb / split stages of 0.36 (the dequantising warps', up to 128
-// tokens) to 0.42 (256 tokens), and a fixed part: filling the ring, the last epilogue, a split's exchange. Measured,
-// 1536 x 4096: 64 rows split 8 ways 9.6, not split 28; 256 rows as 96 CTAs split 2 ways 17.7, as 144 CTAs split 3
-// ways, which are not resident at once, 29; 256 rows gate/up 2 x 4096 x 1536 in tiles of 128 13.9, of 64 22.7.
+// tokens) to 0.42 (256 tokens), and a fixed part: filling the ring, the last epilogue, a split's exchange. A stage
+// costs the same at 64 and 128 tokens, so wide tiles split over more CTAs beat narrow ones. Measured, 1536 x 4096:
+// 64 rows 9.0 split 8 ways, 28 not split; 256 rows 14.1 (tiles of 128, split 4), 14.8 (256, 8), 18.5 (64, 2), 27.9 (64,
+// not split); 512 rows 18.3 (256, 4), 27.9 (128, not split). Gate/up 2 x 4096 x 1536, 256 rows: 14.3 (128, not
+// split), 17.9 (256, 2), 21.0 (64, not split). Of nine such shapes the estimate picks the fastest or one within 7%.
+template <int BN>
+int clusters_at_once(int split, int* out) {
+  const auto kernel = tile_kernel<__nv_bfloat16, BN, false, true, true>;  // the others' resources are the same
+  return kernel_facts(reinterpret_cast<const void*>(kernel), Tile<BN>::kSmemBytes, Tile<BN>::kThreads, split, out);
+}
+
 int choose_shape(TileArgs& p, int sms) {
   double best = 0;
   for (const int bn : {32, 64, 128, 256}) {
     if (bn > 32 && bn / 2 >= p.a.M) break;  // wider than the rows there are
     const int64_t tiles = ((p.a.M + bn - 1) / bn) * p.f_tiles;
-    for (const int split : {1, 2, 3, 4, 8}) {
+    for (const int split : {1, 2, 3, 4, 6, 8}) {
       int at_once = sms;
       if (split > 1) {
-        if (bn > 64 || tiles * split > sms || p.a.n_kb < 4 * split) continue;
-        const auto kernel = tile_kernel<__nv_bfloat16, 64, false, true>;  // the others' resources are the same
-        LEMA_TRY(kernel_facts(reinterpret_cast<const void*>(kernel), Tile<64>::kSmemBytes, Tile<64>::kThreads, split, &at_once));
+        if (tiles * split > sms || p.a.n_kb < 3 * split) continue;
+        LEMA_TRY(bn <= 64 ? clusters_at_once<64>(split, &at_once)
+                          : (bn == 128 ? clusters_at_once<128>(split, &at_once) : clusters_at_once<256>(split, &at_once)));
         if (at_once < 1) continue;
       }
       const double rounds = static_cast<double>((tiles + at_once - 1) / at_once);
       const double stage = 0.36 + 0.0005 * std::max(0, bn - 128);
-      const double us = rounds * ((p.a.n_kb + split - 1) / split) * stage + 0.01 * bn + (split > 1 ? 1.5 : 0);
+      const double us = rounds * ((p.a.n_kb + split - 1) / split) * stage + 0.01 * bn + (split > 1 ? 1.5 + 0.01 * bn : 0);
       if (best == 0 || us < best) {
         best = us;
         p.bn = bn;
