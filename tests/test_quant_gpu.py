@@ -527,3 +527,36 @@ def test_many_rows_give_the_same_bits_every_time(cuda, M, N, K, group, gated):
         other += (call(x, w) != want).sum()
     assert int(other) == 0
     check_status(cuda)
+
+
+@pytest.mark.parametrize("M", [3, 64])
+def test_weights_past_four_gigabytes(cuda, M):
+    """The last block rows of a packed weight of 4.3 GB give what they give alone."""
+    N, K = 131072 + 40, 65536
+    rb = -(-N // 16)
+    packed = torch.randint(-(1 << 31), 1 << 31, (rb, K // 64, 32, 4), dtype=torch.int32, device=cuda)
+    scales = torch.rand(rb, K // 128, 8, 2, device=cuda).mul_(0.01).to(BF16)
+    x = torch.randn(M, K, device=cuda).to(BF16)
+    whole = quant.int4_linear(x, Int4Weight(packed, scales, N, K, 128))
+    first = (rb // 8 - 2) * 8                            # two whole tiles of 8 block rows, and the ragged one
+    n = N - 16 * first
+    tail = quant.int4_linear(x, Int4Weight(packed[first:].contiguous(), scales[first:].contiguous(), n, K, 128))
+    check_status(cuda)
+    assert whole.shape == (M, N)
+    # the same sums; a tile's split of K, and so their order, goes by the number of tiles
+    assert float((whole[:, 16 * first:].double() - tail.double()).norm() / tail.double().norm()) <= 2 * half_step(BF16)
+    assert bool(whole.isfinite().all())
+
+
+def test_rows_of_a_table_past_four_gigabytes(cuda):
+    P, d, cap = 3000, 24, 130_000_000                    # rows from 2.1 to 6.2 GB of a 6.2 GB table
+    st = HashStore(d, groups=P, dtype=BF16, capacity=cap, device=cuda, quant="int8")
+    assert st.nbytes() > 6_000_000_000
+    ref = Dict(P, d, "int8", BF16)
+    rng = np.random.default_rng(12)
+    for T in (1, 5, 1, 1):
+        q, k, v = stream(rng, P, T, d, BF16, span=6)
+        out = torch.empty(P * T, d, dtype=BF16, device=cuda)
+        st.exchange(q.to(cuda), k.to(cuda), v.to(cuda), out, T, 0)
+        assert torch.equal(out.cpu().view(P, T, d), ref.exchange(q, k, v))
+    assert len(st) == sum(len(m) for m in ref.m)
