@@ -90,10 +90,10 @@ class HashStore:
             "cuda", torch.cuda.current_device())
         if self.device.type != "cuda":
             raise LemaError("the B200 store lives in device memory; device must be CUDA")
-        self._index = self.device.index
         self.stride = int(_lib.lib().lema_store_slot_bytes(self.vbytes))
         self.cap = max(16, int(capacity))
         self.table = torch.zeros((self.cap, self.stride), dtype=torch.uint8, device=self.device)
+        self._index = self.table.device.index
         self.counts = torch.zeros(groups, dtype=torch.int64, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._ws = None
@@ -181,6 +181,9 @@ class HashStore:
         dtype = self.dtype
         if (values is not None and values.dtype != dtype) or (out is not None and out.dtype != dtype):
             raise ValueError(f"the store quantises {dtype} rows, got {(out if values is None else values).dtype}")
+        for t in (qcodes, kcodes, values, out):
+            if t is not None and t.get_device() != self._index:
+                raise LemaError(f"the store is on {self.table.device}, got a tensor on {t.device}")
         if rows is None:
             if out is not None and not out.is_contiguous():
                 raise ValueError("values and out must be [n, d_v] (out contiguous), or pass rows=")
@@ -196,11 +199,11 @@ class HashStore:
         args = ("lema_store_exchange_quant", self.table.data_ptr(), self.cap, ROW_FORMATS[self.quant],
                 DTYPE_TAG[dtype], self.d_v, ptr(qcodes), ptr(kcodes), cb, ptr(values), ptr(out), n, T, g0,
                 self.counts.data_ptr() + 8 * g0, self.status.data_ptr(), ptr(ws), 0 if ws is None else ws.numel(),
-                self.seg_groups, self.seg_slots, *rows, phase, stream_handle(self.device))
-        if self._index is None or self._index == torch._C._cuda_getDevice():
+                self.seg_groups, self.seg_slots, *rows, phase, torch._C._cuda_getCurrentRawStream(self._index))
+        if self._index == torch._C._cuda_getDevice():
             call(*args)
         else:
-            with torch.cuda.device(self.device):
+            with torch.cuda.device(self._index):
                 call(*args)
         if check:
             self.check()

@@ -203,3 +203,20 @@ def test_a_quantised_model_counts_copies_and_is_quantised_once():
     assert m.lm_head.weight4.packed is m.lm_head.packed
     with pytest.raises(ValueError, match="group"):
         Transformer(cfg).quantize_weights_(group=48)
+
+
+def test_a_quantised_store_refuses_tensors_of_another_device():
+    # the fields the checks read, without a GPU: nothing below gets as far as a launch
+    from latest_exact_match_attention_b200.cache import Buffers, HashStore, LayerStore
+    st = HashStore.__new__(HashStore)
+    st.dtype, st.d_v, st.groups, st.quant, st._index = torch.bfloat16, 16, 4, "int8", 0
+    st.table = torch.empty(0)
+    k, v = torch.zeros(4, dtype=torch.int32), torch.zeros(4, 16, dtype=torch.bfloat16)
+    with pytest.raises(LemaError, match="the store is on"):
+        st.exchange(k, k, v, torch.empty_like(v), 1, 0)
+    for phase in (1, 2):
+        with pytest.raises(LemaError, match="the store is on"):
+            st.exchange_phase(k, k, v, torch.empty_like(v), 0, phase)
+    view = LayerStore(st, Buffers(torch.bfloat16, None), 0, 4)
+    with pytest.raises(LemaError, match="the store is on"):       # a decode step
+        view.exchange(k.view(1, 4, 1), k.view(1, 4, 1), v.view(1, 4, 1, 16), check=False)

@@ -353,6 +353,20 @@ def test_quantised_store_refuses(cuda):
         st.exchange(k, k, v.to(BF16), torch.empty(4, 16, dtype=BF16, device=cuda), 1, 1)
 
 
+@pytest.mark.parametrize("T", [1, 3])
+def test_quantised_store_refuses_host_tensors(cuda, T):
+    st = HashStore(16, groups=4, dtype=BF16, device="cuda", quant="int8")     # no index: the current device
+    k = torch.zeros(4 * T, dtype=torch.int32, device=cuda)
+    v = torch.ones(4 * T, 16, dtype=BF16, device=cuda)
+    o = torch.empty_like(v)
+    for args in ((k.cpu(), k, v, o), (k, k.cpu(), v, o), (k, k, v.cpu(), o), (k, k, v, o.cpu())):
+        with pytest.raises(LemaError, match="the store is on"):
+            st.exchange(*args, T, 0)
+    assert len(st) == 0
+    st.exchange(k, k, v, o, T, 0)
+    assert len(st) == 4
+
+
 # ------------------------------------------------------------------ together, in the model
 
 
