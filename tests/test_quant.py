@@ -220,3 +220,21 @@ def test_a_quantised_store_refuses_tensors_of_another_device():
     view = LayerStore(st, Buffers(torch.bfloat16, None), 0, 4)
     with pytest.raises(LemaError, match="the store is on"):       # a decode step
         view.exchange(k.view(1, 4, 1), k.view(1, 4, 1), v.view(1, 4, 1, 16), check=False)
+
+
+def test_a_state_dict_brings_its_scales_unrounded():
+    # a model quantised from fp16 weights has fp16 scales, one from fp32 or bf16 weights bf16 scales
+    from latest_exact_match_attention_b200.model import ModelConfig, Transformer
+    torch.manual_seed(2)
+    cfg = ModelConfig(vocab_size=128, depth=1, dim=64, num_heads=4, d_qk=32, d_v=16, dim_ff=128)
+    half = Transformer(cfg).to(torch.float16).quantize_weights_(group=64)
+    wide = Transformer(cfg).quantize_weights_(group=64)
+    for a, b in ((half, wide), (wide, half)):
+        state = {k: v.clone() for k, v in a.state_dict().items()}
+        c = Transformer(cfg).to(b.tok_emb.weight.dtype).quantize_weights_(group=64)
+        assert c.lm_head.scales.dtype == b.lm_head.scales.dtype != state["lm_head.scales"].dtype
+        c.load_state_dict(state)
+        for name in ("lm_head", "blocks.0.attn.o_proj", "blocks.0.mlp.gate_up", "blocks.0.mlp.down"):
+            got, want = c.get_submodule(name), a.get_submodule(name)
+            assert got.scales.dtype == want.scales.dtype and torch.equal(got.scales, want.scales)
+            assert got.weight4.scales is got.scales
