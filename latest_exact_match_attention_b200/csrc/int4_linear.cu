@@ -387,9 +387,9 @@ extern "C" int lema_int4_linear(const void* x, int dtype, int64_t M, int64_t K, 
   a.scale_bf16 = scale_dtype == LEMA_BF16;
   a.vec = aligned(x, 16) && (M == 1 || (ldx * es) % 16 == 0);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // (17 to 32 rows through 50304 x 1536: 43 us here, 32 there; through 1536 x 4096: 5.7 and 8.3)
-  const bool many = M > w4::kMaxRows || (M > w4::kMaxRows / 2 && a.n_rb >= 8 * dev->sms);
-  if (many && w4::tile_ok(a, dtype)) return w4::run_tile(a, dtype, gated != 0, status, s);
+  // Up to 32 rows multiply the codes exactly, whatever the weight's width and the card (17 to 32 rows through 50304 x 1536
+  // would take 32 instead of 43 us in the many-rows kernel, with rounded weights; through 1536 x 4096 8.3 instead of 5.7)
+  if (M > w4::kMaxRows && w4::tile_ok(a, dtype)) return w4::run_tile(a, dtype, gated != 0, status, s);
   if (dtype == LEMA_F32) return w4::run_rows<float>(a, gated != 0, dev->sms, s);
   if (dtype == LEMA_BF16) return w4::run_rows<__nv_bfloat16>(a, gated != 0, dev->sms, s);
   return w4::run_rows<__half>(a, gated != 0, dev->sms, s);
