@@ -459,7 +459,9 @@ int lema_ipc_close(void* ptr, int64_t offset);
  * (i = 1), N counts the features of each, and y = silu(gate) * up with both sums in fp32 (ceil(N / 8)
  * block rows; no residual). Sums are fp32, rounded once to dtype; fp32 inputs keep fp32 accuracy. Up to 32
  * rows, and rows that TMA cannot read (K < 64, ldx or x not a multiple of 16 bytes), multiply the codes
- * exactly and scale each group's fp32 sum; more 16-bit rows multiply s * q rounded once to dtype.
+ * exactly and scale each group's fp32 sum; more 16-bit rows multiply s * q rounded once to dtype's significant bits.
+ * (fp16's range does not bound s * q: a feature's weights are held times a power of two that its largest scale sets, so
+ * only scales below 2^-25 of that one lose bits.)
  * Device-side conditions (a bounded wait that ran out) are OR-ed into status.
  * Replaces: the nn.Linear layers of code/lema/model.py:85-93, 160-175 and 264 for weights held in 4 bits,
  * which the reference does not have.

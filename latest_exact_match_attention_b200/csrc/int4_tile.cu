@@ -19,11 +19,17 @@
 // Here a weight is rounded: s * q (8 + 4 significant bits, or 11 + 4) is rounded once to the rows' 16-bit
 // type, since the tensor core multiplies one type and a tile cannot scale its sums by groups without
 // reading the accumulator back every 32 to 128 inputs. That is half a step a weight, the rounding that a
-// 16-bit checkpoint of the same weights has (fp16's subnormals included).
+// 16-bit checkpoint of the same weights has. fp16 has too short a range for every s q (|s| above 8188, bf16 scales
+// below 2^-14): a feature's weights are held times a power of two that its largest scale sets, so that none is
+// infinite and, of bf16 scales, none of at least 2^-25 of the feature's largest a subnormal; the sums are brought back
+// in fp32. (fp16's own subnormal products are exact, so fp16 scales are only ever brought down.) Both the
+// dequantising and the epilogue's warps read a tile's scales for it first: 0.5 us of 64 rows 1536 x 4096 in groups of 128
+// (9.7 -> 10.2), 2 in groups of 32 (10.1 -> 12.2); 8192 rows gate/up 170 -> 178, 16384 rows 182 -> 185.
 //
 // Every wait is bounded (tcgen05.cuh); a wait that runs out sets the abort flag and
 // LEMA_STATUS_PROBE_LIMIT, and the CTA drains its copies and MMAs and frees its TMEM.
 #include <algorithm>
+#include <type_traits>
 
 #include "int4.cuh"
 #include "tcgen05.cuh"
@@ -88,12 +94,24 @@ template <> struct Pair<__half> {
   __device__ static __forceinline__ float2 to_f2(uint32_t v) { return __half22float2(*reinterpret_cast<const P*>(&v)); }
 };
 
+// fp16 rows: a feature's weights times 2^shift (the head of this file), |s q| 2^shift < 65520. largest: the bits of
+// the feature's largest |s|, fp16 (kSame) or bf16.
+template <bool kSame>
+__device__ __forceinline__ int shift_of(uint32_t largest) {
+  if constexpr (kSame) return min(0, 27 - static_cast<int>(largest >> 10));   // 12 - (exponent - 15)
+  // within fp32's powers of two, and 2^-shift too: what the upper end costs is far below fp16's smallest value
+  return max(-116, min(126, 139 - static_cast<int>(largest >> 7)));           // 12 - (exponent - 127)
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }  // -126 ... 127
+
 // The scale of one row of a fragment: kSame (the scales have the rows' type) as a pair for a 16-bit multiply,
-// whose exact operands' product rounds once, else as fp32.
+// whose exact operands' product rounds once, else as fp32. up: 2^shift of an fp16 row.
 template <typename T, bool kSame> struct RowScale;
 template <typename T> struct RowScale<T, true> {
   uint32_t s;
-  __device__ __forceinline__ RowScale(uint32_t two, int hi, int) : s(hi ? (two >> 16) | (two & 0xFFFF0000u) : (two & 0xFFFFu) | (two << 16)) {}
+  __device__ __forceinline__ RowScale(uint32_t two, int hi, int, uint32_t up) : s(hi ? (two >> 16) | (two & 0xFFFF0000u) : (two & 0xFFFFu) | (two << 16)) {
+    if constexpr (std::is_same<T, __half>::value) s = times(up);
+  }
   __device__ __forceinline__ uint32_t times(uint32_t q) const {
     const typename Pair<T>::P r = __hmul2(*reinterpret_cast<const typename Pair<T>::P*>(&q), *reinterpret_cast<const typename Pair<T>::P*>(&s));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -101,8 +119,10 @@ template <typename T> struct RowScale<T, true> {
 };
 template <typename T> struct RowScale<T, false> {
   float s;
-  __device__ __forceinline__ RowScale(uint32_t two, int hi, int scale_bf16)
-      : s(scale_of(static_cast<uint16_t>(hi ? two >> 16 : two), scale_bf16)) {}
+  __device__ __forceinline__ RowScale(uint32_t two, int hi, int scale_bf16, uint32_t up)
+      : s(scale_of(static_cast<uint16_t>(hi ? two >> 16 : two), scale_bf16)) {
+    if constexpr (std::is_same<T, __half>::value) s *= __uint_as_float(up);
+  }
   __device__ __forceinline__ uint32_t times(uint32_t q) const {
     const float2 v = Pair<T>::to_f2(q);
     return Pair<T>::from_f(v.x * s, v.y * s);
@@ -242,8 +262,18 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 3 * kStages + 5);
   volatile uint32_t* s_abort = s_tmem + 1;
 
+  constexpr bool kShift = std::is_same<T, __half>::value;
   const Args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // what brings the sums of row `row_in` of tile f_tile back (kShift): one over its feature's power of two
+  auto back = [&](int f_tile, int row_in) {
+    const int rb = min(f_tile * kTileBlocks + (row_in >> 4), a.n_rb - 1);
+    const uint16_t* s = a.scales + static_cast<int64_t>(rb) * a.n_groups * 16 + row_of(row_in & 7) * 2 + ((row_in >> 3) & 1);
+    uint32_t largest = 0;
+#pragma unroll 8
+    for (int grp = 0; grp < a.n_groups; ++grp) largest = max(largest, __ldg(s + grp * 16) & 0x7FFFu);
+    return power_of_two(-shift_of<kSame>(largest));
+  };
   // this CTA's tiles, and its share of their K blocks
   // (grid: x the CTAs of a cluster, y the tiles; read as blockIdx and gridDim everywhere, which keeps the loops'
   // counters and the MMA's descriptors in uniform registers: copies of them cost 8% at 16384 rows)
@@ -352,6 +382,8 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
     int acc = 0;
     uint32_t aph = 0;
     for (int64_t tile = blockIdx.y; !kSplit && tile < p.n_tiles; tile += gridDim.y) {
+      float times = 1.f;
+      if constexpr (kShift) times = back(static_cast<int>(tile % p.f_tiles), quarter * 32 + lane);
       if (!warp_wait(accf_bar(acc), aph, s_abort, p.status, p.wait_ns)) break;
       tc_fence_after();
       const int64_t m0 = (tile / p.f_tiles) * p.bn;
@@ -363,7 +395,7 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
         tmem_load32(tmem_base + lane_base + static_cast<uint32_t>(acc * BN + j), r);
         float v[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(r[c]);
+        for (int c = 0; c < 32; ++c) v[c] = kShift ? __uint_as_float(r[c]) * times : __uint_as_float(r[c]);
         finish<T, kGated, 32>(p, row, m, v);
       }
       tc_fence_before();
@@ -407,6 +439,29 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
       };
       int kb = skip;
       if (kb < kb1) fetch(kb);
+      uint32_t shift[kMine][2];  // 2^shift of rows g and g + 8 (kShift): a pair of fp16, or fp32
+      if constexpr (kShift) {
+        uint32_t top[kMine];  // of rows g and g + 8, the lanes of a row each a quarter of its groups
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) top[b] = 0;
+#pragma unroll (16 / kMine)
+        for (int grp = t; grp < a.n_groups; grp += 4)
+#pragma unroll
+          for (int b = 0; b < kMine; ++b) top[b] = __vmaxu2(top[b], __ldg(sp[b] + grp * 8) & 0x7FFF7FFFu);
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) {
+          top[b] = __vmaxu2(top[b], __shfl_xor_sync(0xFFFFFFFFu, top[b], 1));
+          top[b] = __vmaxu2(top[b], __shfl_xor_sync(0xFFFFFFFFu, top[b], 2));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int e = shift_of<kSame>(i ? top[b] >> 16 : top[b] & 0xFFFFu);
+            if constexpr (kSame)
+              shift[b][i] = Pair<T>::from_f(power_of_two(e), power_of_two(e));
+            else
+              shift[b][i] = __float_as_uint(power_of_two(e));
+          }
+        }
+      }
       for (; kb < kb1; kb += kSets) {
         uint4 w[kMine];
         uint32_t sc[kMine][2];
@@ -429,7 +484,7 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
             Unpack<T>::run(words[2 * h + 1], f1);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const RowScale<T, kSame> rs(sc[b][h], i, a.scale_bf16);
+              const RowScale<T, kSame> rs(sc[b][h], i, a.scale_bf16, kShift ? shift[b][i] : 0u);
               v[i][h].x = rs.times(f0[i]);
               v[i][h].y = rs.times(f0[i + 2]);
               v[i][h].z = rs.times(f1[i]);
@@ -473,7 +528,9 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
       return sbase + static_cast<uint32_t>(((src < dst ? src : src - 1) * mine + k) * TL::kUnitBytes + row_in * 16);
     };
     bool ok = false;
+    float times = 1.f;
     if (live) {
+      if constexpr (kShift) times = back(static_cast<int>(blockIdx.y % p.f_tiles), row_in);
       ok = warp_wait(accf_bar(0), 0, s_abort, p.status, p.wait_ns);
       tc_fence_after();
     }
@@ -522,6 +579,10 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
 #pragma unroll
             for (int c = 0; c < 4; ++c) v[4 * h + c] += f[c];
           }
+        }
+        if constexpr (kShift) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] *= times;
         }
         finish<T, kGated, 8>(p, row, m0 + u * 8, v);
       }

@@ -51,3 +51,69 @@ def test_up_to_32_rows_multiply_codes_exactly(cuda, M, block_rows_of_each_sm, dt
         parts = torch.cat([call(x[i:i + 8].contiguous(), packed) for i in range(0, M, 8)])
         assert torch.equal(call(x, packed), parts)
     check_status(cuda)
+
+
+def check_products(x, s_dtype, spread, M, N, K, group, seed, dev, residual):
+    """fp16 rows against 64-bit sums, gate/up pairs too. spread [N, groups]: powers of two of the scales."""
+    c, s = weight(N, K, group, s_dtype, seed, dev)
+    s = (s.float() / s.float().abs().amax() * 2.0 ** spread.to(dev)).to(s_dtype)
+    w = dense64(c, s, group)
+    # fp32 sums (2^-23 of the magnitudes an addition), half a step of 2^-11 a weight, or, for scales far below the
+    # feature's largest, three times half a step of fp16's subnormals under its power of two, 2^-25 2^(e - 12)
+    low = 3 * 2.0 ** (torch.floor(torch.log2(s.double().abs().amax(1))) - 12 - 25)
+    mag = x.double().abs() @ w.abs().t()
+    off = mag * ((K + 8) * 2.0 ** -23 + 2.0 ** -11) + x.double().abs().sum(1, keepdim=True) * low
+    ref = x.double() @ w.t()
+    r = torch.randn(M, N, generator=torch.Generator().manual_seed(seed)).half().to(dev) if residual else None
+    got = quant.int4_linear(x, Int4Weight.pack(c, s, group), residual=r)
+    check_status(dev)
+    full = ref if r is None else ref + r.double()
+    bound = off + 2.0 ** -11 * (full.abs() + off) + 2.0 ** -25        # the output's rounding, subnormals too
+    err = (got.double() - full).abs()
+    ok = full.abs() + off < 65504                                     # what fp16 holds; past it infinities
+    assert bool((err <= bound)[ok].all()), f"{float((err / bound)[ok].nan_to_num(nan=1e9).max()):.3g} of the bound"
+    assert float(ok.double().mean()) > 0.99
+    past = full.abs() - off > 65520
+    assert torch.equal(got[past], torch.sign(full[past]).half() * float("inf"))
+    gu = quant.int4_swiglu(x, Int4Weight.pack_gate_up(c, s, c, s, group))
+    want = ref * torch.sigmoid(ref) * ref
+    ok = want.abs() + 1.1 * off * (2 * ref.abs() + off) < 60000
+    bound = 1.1 * off * (ref.abs() + off) + ref.abs() * off
+    bound = bound + (2.0 ** -11 + 2.0 ** -17) * (want.abs() + bound) + 2.0 ** -25
+    assert bool(((gu.double() - want).abs() <= bound)[ok].all()) and int(ok.sum()) > 0
+
+
+@pytest.mark.parametrize("M,N,K,group", [(33, 100, 320, 64), (64, 256, 4096, 128), (300, 272, 1096, 32), (2100, 1000, 200, 32)])
+@pytest.mark.parametrize("s_dtype", [BF16, F16])
+@pytest.mark.parametrize("kind", ["large", "small", "both"])
+def test_fp16_rows_through_weights_beyond_fp16(cuda, kind, s_dtype, M, N, K, group):
+    """Weights s q above 65504 and, with bf16 scales, far below fp16's smallest, in tiles alone and with K split: sums that
+    fp16 holds come out, within the rounding of the weights' significant bits. Features differ, and in "both" the
+    groups of a feature."""
+    g = torch.Generator().manual_seed(M)
+    groups = -(-K // group)
+    top = 15 if s_dtype == F16 else 20
+    if kind == "large":
+        spread, size = torch.randint(8, top + 1, (N, 1), generator=g).expand(N, groups).double(), 2.0 ** -13
+    elif kind == "small":
+        spread, size = torch.randint(-12 if s_dtype == F16 else -26, -6, (N, 1), generator=g).expand(N, groups).double(), 2.0 ** 6
+    else:
+        spread, size = torch.randint(-8, top + 1, (N, groups), generator=g).double(), 2.0 ** -13
+    x = (torch.randn(M, K, generator=g).clamp(-4, 4) * size).half().to(cuda)
+    check_products(x, s_dtype, spread, M, N, K, group, M + K, cuda, residual=M % 2 == 1)
+
+
+@pytest.mark.parametrize("M", [3, 40, 400])
+@pytest.mark.parametrize("s_dtype", [BF16, F16])
+def test_features_without_a_usable_scale_touch_only_themselves(cuda, s_dtype, M):
+    """All-zero, infinite and NaN scales in fp16 rows' weights, few rows and tiles alike."""
+    N, K, group = 72, 256, 64
+    c, s = weight(N, K, group, s_dtype, 1, cuda)
+    c = torch.where(c == 0, torch.ones_like(c), c)
+    x = torch.rand(M, K, generator=torch.Generator().manual_seed(M)).add(0.5).half().to(cuda)
+    clean = quant.int4_linear(x, Int4Weight.pack(c, s, group))
+    s[5], s[17, 2], s[40, 0] = 0, float("inf"), float("nan")
+    got = quant.int4_linear(x, Int4Weight.pack(c, s, group))
+    others = [n for n in range(N) if n not in (5, 17, 40)]
+    assert torch.equal(got[:, others], clean[:, others])
+    assert bool((got[:, 5] == 0).all()) and not bool(got[:, [17, 40]].isfinite().any())
