@@ -370,9 +370,6 @@ class Transformer(nn.Module):
     def n_params(self, embedding: bool = True) -> int:
         """Parameter count (4-bit weights counted as weights); embedding=False leaves out the token
         embedding and the head."""
-        n = sum(p.numel() for p in self.parameters())
-        n += sum(m.n_weights() for m in self.modules() if isinstance(m, Int4Module))
-        if embedding:
-            return n
-        head = self.lm_head
-        return n - self.tok_emb.weight.numel() - (head.n_weights() if isinstance(head, Int4Module) else head.weight.numel())
+        skip = set() if embedding else {id(self.tok_emb.weight), id(self.lm_head), id(getattr(self.lm_head, "weight", None))}
+        return (sum(p.numel() for p in self.parameters() if id(p) not in skip)
+                + sum(m.n_weights() for m in self.modules() if isinstance(m, Int4Module) and id(m) not in skip))
