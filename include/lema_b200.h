@@ -318,7 +318,7 @@ int lema_store_exchange_phase(void* table, int64_t cap, int64_t vbytes, const vo
  *   LEMA_ROWS_INT8  s = fl32(amax / 127) of the row, code = clamp(rne(v / s), -127, 127)
  *   LEMA_ROWS_FP8   s = the smallest power of two with amax / s <= 448 (2^-126 at least), code = e4m3(v / s)
  *   LEMA_ROWS_INT4  s = fl32(amax / 7) of each 32 values, code = clamp(rne(v / s), -7, 7)
- * (rne: the exact quotient rounded, ties to even); the value given back is fl32(s * code), saturated to
+ * (rne: the exact quotient rounded, ties to even; 0 where s rounds to 0); the value given back is fl32(s * code), saturated to
  * dtype's largest finite value, rounded to dtype. An infinity or a NaN makes its scale, and so every value of its group, NaN. A row found
  * inside the same call (T > 1) is given back as the same numbers a later call would find, so any
  * chunking of a sequence gives the same results. The table is cap slots of

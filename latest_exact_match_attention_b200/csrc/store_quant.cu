@@ -149,8 +149,9 @@ __device__ __forceinline__ Frag<F> quantise(const float (&f)[8], const Lane<G>& 
   } else {
     constexpr float kTop = F == LEMA_ROWS_INT8 ? 127.f : 7.f;
     q.s = __fdiv_rn(__uint_as_float(m), kTop);
-    // rows near the bottom of fp32's range are lifted, so that 1 / s exists
-    const float lift = q.s < 0x1p-100f ? 0x1p100f : 1.f;
+    // rows near the bottom of fp32's range are lifted, so that 1 / s exists; where the scale itself rounds to 0 (fp32 rows
+    // below 64 of the smallest steps there are, int4: 4) the codes are 0
+    const float lift = q.s < 0x1p-100f ? (q.s > 0.f ? 0x1p100f : 0.f) : 1.f;
     const float s = q.s * lift;
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
     uint32_t w[2] = {0, 0};

@@ -5,7 +5,8 @@ import torch
 
 from latest_exact_match_attention_b200 import quant
 from latest_exact_match_attention_b200._lib import check_status
-from latest_exact_match_attention_b200.quant import Int4Weight
+from latest_exact_match_attention_b200.cache import HashStore
+from latest_exact_match_attention_b200.quant import Int4Weight, dequantize_rows, quantize_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +118,41 @@ def test_features_without_a_usable_scale_touch_only_themselves(cuda, s_dtype, M)
     others = [n for n in range(N) if n not in (5, 17, 40)]
     assert torch.equal(got[:, others], clean[:, others])
     assert bool((got[:, 5] == 0).all()) and not bool(got[:, [17, 40]].isfinite().any())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8", "int4"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [40, 7])
+def test_held_bytes_are_those_of_quantize_rows(cuda, fmt, dtype, d):
+    """Byte for byte, and the values given back bit for bit (NaNs aside: any NaN): random rows, zeros of both signs, the ends
+    of the type, and amplitudes so small that a scale is a subnormal or zero."""
+    fi = torch.finfo(dtype)
+    tiny = fi.smallest_normal * fi.eps
+    g = torch.Generator().manual_seed(d)
+    rows = torch.randn(300, d, generator=g) * torch.exp(3 * torch.randn(300, 1, generator=g))
+    sign = torch.where(torch.rand(64, d, generator=g) < 0.5, -1.0, 1.0)
+    steps = torch.arange(1, 65)[:, None] * torch.rand(64, d, generator=g).add(0.01)      # amax of 1 to 64 subnormal steps
+    more = [rows, sign * steps.round() * tiny, torch.zeros(1, d), -torch.zeros(1, d), torch.full((1, d), -tiny),
+            torch.full((1, d), 63 * tiny), torch.full((1, d), -64 * tiny), torch.full((1, d), -fi.max), rows[:8] * fi.smallest_normal,
+            torch.linspace(-190, 190, d)[None] * tiny]
+    rows = torch.cat(more).to(dtype)
+    bad = rows[:3].clone()
+    bad[0, 1], bad[1, d - 1], bad[2, 0] = float("inf"), float("nan"), float("-inf")
+    rows = torch.cat([rows, bad])
+    P = rows.shape[0]
+    code = torch.arange(P, dtype=torch.int32, device=cuda)
+    st = HashStore(d, groups=P, dtype=dtype, capacity=4 * P, device=cuda, quant=fmt)
+    out = torch.empty(P, d, dtype=dtype, device=cuda)
+    for _ in range(2):
+        st.exchange(code, code, rows.to(cuda), out, 1, 0)
+    want = quantize_rows(rows, fmt)
+    state = st.table.view(-1)[: 16 * st.cap].view(torch.int64).view(st.cap, 2)[:, 1].cpu()
+    live = (state >= 2).nonzero().squeeze(1)
+    held = torch.empty_like(want)
+    held[state[live] - 2] = st.table.view(-1)[16 * st.cap:].view(st.cap, -1)[live.to(cuda)].cpu()
+    assert live.numel() == P
+    wrong = (held != want).any(1).nonzero().squeeze(1).tolist()
+    assert not wrong, f"row {wrong[0]}: {rows[wrong[0]].tolist()}"
+    back = dequantize_rows(want, fmt, d, dtype)
+    ints = torch.int32 if dtype == F32 else torch.int16
+    assert bool(((out.cpu().view(ints) == back.view(ints)) | (out.cpu().isnan() & back.isnan())).all())
