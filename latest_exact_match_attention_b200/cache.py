@@ -219,17 +219,21 @@ class HashStore:
         n = codes.numel()
         if g0 < 0 or g0 + n > self.groups:
             raise ValueError(f"groups [{g0}, {g0 + n}) outside the store's {self.groups}")
+        one = phase == 1
+        rows = out if one else values
+        if rows.numel() != n * self.d_v or rows.shape[-1] != self.d_v:
+            raise ValueError(f"rows must be [n, d_v] = [{n}, {self.d_v}], got {tuple(rows.shape)}")
         if self.quant is not None:
-            one = phase == 1
-            rows = out if one else values
-            if rows.numel() != n * self.d_v or rows.shape[-1] != self.d_v:
-                raise ValueError(f"rows must be [n, d_v] = [{n}, {self.d_v}], got {tuple(rows.shape)}")
             return self._exchange_quant(qcodes if one else None, None if one else kcodes, None if one else values,
                                         out if one else None, n, 1, g0, None, phase, False)
+        if rows.element_size() * self.d_v != self.vbytes:
+            raise ValueError(f"value rows of {rows.element_size() * self.d_v} bytes, the store holds {self.vbytes}")
+        if one and not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+        codes, rows = codes.contiguous(), rows.contiguous()
         call("lema_store_exchange_phase", ptr(self.table), self.cap, self.vbytes,
-             ptr(qcodes) if phase == 1 else None, ptr(kcodes) if phase == 2 else None,
-             code_bytes_of(codes), ptr(values) if phase == 2 else None,
-             ptr(out) if phase == 1 else None, n, g0, ptr(self.counts) + 8 * g0, ptr(self.status),
+             ptr(codes) if one else None, None if one else ptr(codes), code_bytes_of(codes),
+             None if one else ptr(rows), ptr(rows) if one else None, n, g0, ptr(self.counts) + 8 * g0, ptr(self.status),
              self.seg_groups, self.seg_slots, phase, stream_handle(self.device))
 
     def dump(self):
