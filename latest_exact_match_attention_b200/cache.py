@@ -361,10 +361,10 @@ class LayerStore:
         `[B, H, T, d_v]` like `v`, zeros where nothing matched."""
         st = self.store
         if (st.quant is not None and v.dim() == 4 and v.shape[2] == 1 and self.buffers.codes_hook is None
-                and not self.persistent_out):
+                and not self.persistent_out and kc.dtype == qc.dtype):
             # a decode step on quantised rows: the same checks and one call, without the staging object
             n = qc.numel()
-            if n != self.partitions or kc.numel() != n or kc.dtype != qc.dtype or v.numel() != n * st.d_v or v.shape[3] != st.d_v:
+            if n != self.partitions or kc.numel() != n or v.numel() != n * st.d_v or v.shape[3] != st.d_v:
                 raise ValueError(f"a step's codes and values must be [B, H, 1] and [B, H, 1, {st.d_v}] of {self.partitions} "
                                  f"partitions, got {tuple(qc.shape)}, {tuple(kc.shape)} and {tuple(v.shape)}")
             out = v.new_empty(v.shape)

@@ -3,6 +3,7 @@ needed)."""
 import pytest
 import torch
 
+from latest_exact_match_attention_b200._lib import LemaError
 from latest_exact_match_attention_b200.model import ModelConfig, Transformer
 
 
@@ -53,3 +54,12 @@ def test_half_a_step_on_raw_rows_checks_their_bytes_and_layout():
             st.exchange_phase(k, k, v, v.clone(), 0, phase)
     with pytest.raises(ValueError, match="contiguous"):
         st.exchange_phase(k, k, v.bfloat16(), torch.zeros(16, 4, dtype=torch.bfloat16).t(), 0, 1)
+
+
+def test_a_step_with_key_codes_of_the_other_width_gets_as_far_as_the_device():
+    from latest_exact_match_attention_b200.cache import Buffers, LayerStore
+    view = LayerStore(store_without_a_gpu("int8"), Buffers(torch.bfloat16, None), 0, 4)
+    k, v = torch.zeros(1, 4, 1, dtype=torch.int32), torch.zeros(1, 4, 1, 16, dtype=torch.bfloat16)
+    for q, k2 in ((k, k.long()), (k.long(), k), (k, k)):
+        with pytest.raises(LemaError, match="the store is on"):
+            view.exchange(q, k2, v, check=False)

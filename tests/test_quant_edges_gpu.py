@@ -5,7 +5,8 @@ import torch
 
 from latest_exact_match_attention_b200 import quant
 from latest_exact_match_attention_b200._lib import check_status
-from latest_exact_match_attention_b200.cache import HashStore
+from latest_exact_match_attention_b200.cache import HashStore, LemaCache
+from latest_exact_match_attention_b200.model import ModelConfig
 from latest_exact_match_attention_b200.quant import Int4Weight, dequantize_rows, quantize_rows
 
 pytestmark = pytest.mark.gpu
@@ -156,3 +157,16 @@ def test_held_bytes_are_those_of_quantize_rows(cuda, fmt, dtype, d):
     back = dequantize_rows(want, fmt, d, dtype)
     ints = torch.int32 if dtype == F32 else torch.int16
     assert bool(((out.cpu().view(ints) == back.view(ints)) | (out.cpu().isnan() & back.isnan())).all())
+
+
+@pytest.mark.parametrize("quant", [None, "int8"])
+def test_a_step_takes_key_codes_of_the_other_width(cuda, quant):
+    """As a prompt's chunk and a store of raw rows do: key codes become the query codes' type."""
+    cfg = ModelConfig(vocab_size=128, depth=1, dim=64, num_heads=4, d_qk=32, d_v=16)
+    c = [LemaCache(cfg, dtype=BF16, batch=1, max_cache_len=40, device=cuda, quant=quant) for _ in range(2)]
+    g = torch.Generator().manual_seed(0)
+    for _ in range(20):
+        q, k = (torch.randint(0, 5, (1, 4, 1), generator=g).to(torch.int32).to(cuda) for _ in range(2))
+        v = torch.randn(1, 4, 1, 16, generator=g).to(BF16).to(cuda)
+        assert torch.equal(c[0].layer(0).exchange(q, k, v), c[1].layer(0).exchange(q, k.long(), v))
+    assert torch.equal(c[0].counts(), c[1].counts())
