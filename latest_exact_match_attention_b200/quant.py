@@ -234,7 +234,13 @@ class Int4Module(nn.Module):
         super()._apply(fn, recurse)
         if self.scales.dtype != before.dtype:
             self.scales = before.to(self.scales.device)
+        self._weight = None     # it holds the buffers that a move has just replaced
         return self
+
+    def __setattr__(self, name, value):
+        super().__setattr__(name, value)
+        if name in ("packed", "scales"):
+            super().__setattr__("_weight", None)
 
     def _load_from_state_dict(self, state_dict, prefix, *args):
         # a state dict's scales come in with their own 16-bit type: cast to this module's, weights would change
@@ -247,7 +253,7 @@ class Int4Module(nn.Module):
     def weight4(self) -> Int4Weight:
         """The buffers as an Int4Weight (made anew when the module's buffers have been replaced)."""
         w, packed, scales = self._weight, self.packed, self.scales
-        if w.packed is not packed or w.scales is not scales:
+        if w is None or w.packed is not packed or w.scales is not scales:
             w = self._weight = Int4Weight(packed, scales, self.n, self.k, self.group, self.gated)
         return w
 

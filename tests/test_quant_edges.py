@@ -5,6 +5,7 @@ import torch
 
 from latest_exact_match_attention_b200._lib import LemaError
 from latest_exact_match_attention_b200.model import ModelConfig, Transformer
+from latest_exact_match_attention_b200.quant import Int4Module
 
 
 def small(**kw):
@@ -63,3 +64,24 @@ def test_a_step_with_key_codes_of_the_other_width_gets_as_far_as_the_device():
     for q, k2 in ((k, k.long()), (k.long(), k), (k, k)):
         with pytest.raises(LemaError, match="the store is on"):
             view.exchange(q, k2, v, check=False)
+
+
+def test_buffers_that_a_module_gave_up_are_freed():
+    import gc
+    import weakref
+    moves = [lambda m: m._apply(torch.clone), lambda m: m.to("meta"), lambda m: m.half(),
+             lambda m: m.load_state_dict({k: v.clone() for k, v in m.state_dict().items()}, assign=True),
+             lambda m: [setattr(x, "packed", x.packed.clone()) or setattr(x, "scales", x.scales.clone())
+                        for x in m.modules() if isinstance(x, Int4Module)]]
+    for move in moves:
+        m = small().quantize_weights_(group=64)
+        held = [x for x in m.modules() if isinstance(x, Int4Module)]
+        assert len(held) == 2 * 4 + 1
+        for x in held:
+            x.weight4                                    # as a forward would have
+        before = [(name, weakref.ref(b), b.data_ptr()) for x in held for name, b in (("packed", x.packed), ("scales", x.scales))]
+        move(m)
+        gc.collect()
+        kept = {b.data_ptr() for x in held for b in x.buffers()}
+        assert all(ref() is None or at in kept for _, ref, at in before)
+        assert all(x.weight4.packed is x.packed and x.weight4.scales is x.scales for x in held)
