@@ -245,7 +245,8 @@ class Int4Module(nn.Module):
     def _load_from_state_dict(self, state_dict, prefix, *args):
         # a state dict's scales come in with their own 16-bit type: cast to this module's, weights would change
         s = state_dict.get(prefix + "scales")
-        if s is not None and s.dtype != self.scales.dtype and s.dtype in (torch.bfloat16, torch.float16):
+        if (s is not None and s.shape == self.scales.shape and s.dtype != self.scales.dtype
+                and s.dtype in (torch.bfloat16, torch.float16)):
             self.scales = self.scales.to(s.dtype)
         super()._load_from_state_dict(state_dict, prefix, *args)
 

@@ -85,3 +85,16 @@ def test_buffers_that_a_module_gave_up_are_freed():
         kept = {b.data_ptr() for x in held for b in x.buffers()}
         assert all(ref() is None or at in kept for _, ref, at in before)
         assert all(x.weight4.packed is x.packed and x.weight4.scales is x.scales for x in held)
+
+
+def test_a_state_dict_of_another_group_leaves_the_scales():
+    m = small().quantize_weights_(group=64)
+    other = small().to(torch.float16).quantize_weights_(group=32).state_dict()      # fp16 scales, twice as many
+    before = {k: v.clone() for k, v in m.state_dict().items() if k.endswith("scales")}
+    with pytest.raises(RuntimeError, match="scales"):
+        m.load_state_dict(other)
+    after = m.state_dict()
+    for k, v in before.items():
+        if v.shape != other[k].shape:
+            assert after[k].dtype == torch.bfloat16 and torch.equal(after[k], v)
+    assert any(v.shape != other[k].shape for k, v in before.items())
