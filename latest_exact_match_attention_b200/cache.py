@@ -97,7 +97,6 @@ class HashStore:
         self.counts = torch.zeros(groups, dtype=torch.int64, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._ws = None
-        self._ws_held = []     # workspaces that captured graphs still use
         # segments > 1: each run of groups/segments groups (a layer, for LemaCache) has its
         # home slots in its own 1/segments of the table; results are the same either way
         segments = max(1, min(int(segments), groups, self.cap))
@@ -115,21 +114,19 @@ class HashStore:
         return len(self) / self.cap
 
     def reserve(self, n: int, T: int, code_bytes: int = 8) -> None:
-        """Allocate the exchange workspace for n items in chunks of T ahead of time (before a
-        CUDA graph capture, say)."""
+        """Allocate the exchange workspace for n items in chunks of T ahead of time. (A call that is
+        being captured into a CUDA graph takes its workspace from the graph's memory.)"""
         self._workspace(n, T, code_bytes)
 
     def _workspace(self, n: int, T: int, code_bytes: int):
         need = int(_lib.lib().lema_store_workspace_bytes(n, T, code_bytes))
         if need == 0:
             return None
+        if torch.cuda.is_current_stream_capturing():
+            # the graph's own memory: its replays share it with no other graph or call, and it goes with the graph
+            return torch.empty(need, dtype=torch.uint8, device=self.device)
         if self._ws is None or self._ws.numel() < need:
-            if torch.cuda.is_current_stream_capturing():
-                raise LemaError("store workspace must be reserved before graph capture "
-                                "(HashStore.reserve)")
             self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        if torch.cuda.is_current_stream_capturing() and not any(self._ws is w for w in self._ws_held):
-            self._ws_held.append(self._ws)      # a replay uses it even after a larger call replaced it
         return self._ws
 
     def exchange(self, qcodes: torch.Tensor, kcodes: torch.Tensor, values: torch.Tensor,

@@ -1,5 +1,8 @@
 """Quantised serving where its kernels meet: the rule that picks one, the ends of 16-bit ranges, and the bytes a
 quantised store holds."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -170,3 +173,49 @@ def test_a_step_takes_key_codes_of_the_other_width(cuda, quant):
         v = torch.randn(1, 4, 1, 16, generator=g).to(BF16).to(cuda)
         assert torch.equal(c[0].layer(0).exchange(q, k, v), c[1].layer(0).exchange(q, k.long(), v))
     assert torch.equal(c[0].counts(), c[1].counts())
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_a_captured_chunk_has_a_workspace_of_its_own(cuda, fmt):
+    """It needs no reservation, replays after a larger eager call and beside another graph, and goes with the graph."""
+    P, T, d = 4, 64, 24
+    g = torch.Generator().manual_seed(1)
+
+    def items(t, at):
+        q, k = (torch.randint(at, at + 300, (P * t,), generator=g).to(torch.int32).to(cuda) for _ in range(2))
+        return q, k, torch.randn(P * t, d, generator=g).to(BF16).to(cuda)
+
+    def store():
+        return HashStore(d, groups=P, dtype=BF16, capacity=40000, device=cuda, quant=fmt)
+
+    sets = [items(T, 0), items(T, 1000), items(40 * T, 5000)]
+    st, ref = store(), store()
+    warm = [torch.empty_like(s[2]) for s in sets]
+    st.exchange(*sets[0], warm[0], T, 0)                             # the kernels' first launches are not captured
+    old = weakref.ref(st._ws)
+    outs, graphs = [torch.empty_like(s[2]) for s in sets], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            st.exchange(*sets[i], outs[i], T, 0, check=False)
+    st.exchange(*sets[2], outs[2], 40 * T, 0)
+    gc.collect()
+    assert old() is None                                             # replaced by the larger call's, held by no graph
+    for _ in range(2):
+        for gr in graphs:
+            gr.replay()
+    for i in (0, 2, 0, 1, 0, 1):
+        ref.exchange(*sets[i], warm[i], T if i < 2 else 40 * T, 0)
+    st.check()
+    assert all(torch.equal(a, b) for a, b in zip(outs, warm))
+    assert torch.equal(st.counts, ref.counts)
+    fresh = store()                                                  # captured before any eager call of its own
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fresh.exchange(*sets[0], outs[0], T, 0, check=False)
+    other = store()
+    for _ in range(2):
+        graph.replay()
+        other.exchange(*sets[0], warm[0], T, 0)
+    fresh.check()
+    assert torch.equal(outs[0], warm[0]) and torch.equal(fresh.counts, other.counts)
