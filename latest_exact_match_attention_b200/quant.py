@@ -27,7 +27,14 @@ __all__ = ["Int4Weight", "Int4Linear", "Int4SwiGLU", "quantize_weight", "int4_li
            "ROW_FORMATS", "row_bytes", "quantize_rows", "dequantize_rows"]
 
 GROUPS = (32, 64, 128)
-COPY_ROWS = 128     # more unaligned 16-bit rows than this are worth a copy for the tcgen05 kernel
+FEW_ROWS = 32       # up to this many rows have a kernel of their own, which reads rows of any alignment
+# Unaligned 16-bit rows: above FEW_ROWS that kernel takes them too, 32 at a time with checked loads; a call on an aligned
+# copy takes about 20 us of host time and 9 to 25 on the device. Rows are copied where there are many of them and where
+# blocks of 16 x 64 weights times 32-row tiles exceed COPY_WORK (fp16, as they are / copied, us a call): 37 rows
+# 1000 x 1100 (2268) 10.5 / 19.9, 64 rows 1000 x 2501 (5040) 15.9 / 20.1, 33 rows 8192 x 333 (6144) 17.3 / 19.7, 128 rows
+# 4096 x 333 (6144) 22.1 / 19.7, 96 rows 1000 x 2501 (7560) 30.1 / 20.3, 33 rows 50304 x 1100 (113184) 173 / 29, 128 rows 515 / 31.
+COPY_ROWS = 128
+COPY_WORK = 6000
 
 # ------------------------------------------------------------------ 4-bit weights
 
@@ -164,9 +171,9 @@ def _product(name: str, x: torch.Tensor, w: Int4Weight, residual: torch.Tensor |
         if x.stride(1) != 1 or (x.shape[0] > 1 and ldx < k):
             x, ldx = x.contiguous(), k
     M = x.numel() // k
-    if M > COPY_ROWS and tag != F32 and k >= 64 and ((ldx | x.data_ptr() >> 1) & 7):
-        # rows that the many-rows kernel cannot load in 16-byte pieces: an aligned copy of them (fewer take the
-        # few-rows kernel as they are: 37 rows of 1100 in 13 us, less than the host time of a copy)
+    if (M > FEW_ROWS and ((ldx | x.data_ptr() >> 1) & 7) and tag != F32 and k >= 64
+            and (M > COPY_ROWS or (packed.numel() >> 7) * ((M + 31) >> 5) > COPY_WORK)):
+        # rows that the many-rows kernel cannot load in 16-byte pieces: an aligned copy of them
         ldx = -(-k // 8) * 8
         rows = x.new_empty((M, ldx))
         rows[:, :k].copy_(x if x.dim() == 2 else x.view(M, k))

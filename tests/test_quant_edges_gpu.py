@@ -219,3 +219,35 @@ def test_a_captured_chunk_has_a_workspace_of_its_own(cuda, fmt):
         other.exchange(*sets[0], warm[0], T, 0)
     fresh.check()
     assert torch.equal(outs[0], warm[0]) and torch.equal(fresh.counts, other.counts)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,K", [(8192, 333), (2048, 1501), (50304, 100)])
+@pytest.mark.parametrize("M", [33, 64, 96, 128])
+def test_unaligned_rows_through_wide_weights_give_the_bits_of_aligned_ones(cuda, M, N, K, dtype):
+    """The same kernel as aligned rows take, plain and gate/up, whatever makes them unaligned."""
+    c, s = weight(N, K, 64, dtype, M, cuda)
+    w = Int4Weight.pack(c, s, 64)
+    gu = Int4Weight.pack_gate_up(c[: N // 2], s[: N // 2], c[N // 2:], s[N // 2:], 64)
+    ka = -(-K // 8) * 8
+    room = torch.randn(M, ka, generator=torch.Generator().manual_seed(K)).to(dtype).to(cuda)
+    x = room[:, :K]                                                  # 16-byte aligned rows
+    flat = torch.empty(M * ka + 1, dtype=dtype, device=cuda)[1:].view(M, ka)
+    flat.copy_(room)
+    for call, packed in ((quant.int4_linear, w), (quant.int4_swiglu, gu)):
+        want = call(x, packed)
+        assert torch.equal(call(x.contiguous(), packed), want) and torch.equal(call(flat[:, :K], packed), want)
+    check_status(cuda)
+
+
+@pytest.mark.parametrize("M", [17, 32, 33, 37, 100])
+def test_unaligned_rows_through_narrow_weights(cuda, M):
+    """Too little work for a copy: exact products still."""
+    N, K = 200, 333
+    c, s = weight(N, K, 64, F16, M, cuda)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(K)).half().to(cuda)
+    got = quant.int4_linear(x, Int4Weight.pack(c, s, 64))
+    w = dense64(c, s, 64)
+    ref = x.double() @ w.t()
+    off = (x.double().abs() @ w.abs().t()) * (K + 8) * 2.0 ** -23
+    assert bool(((got.double() - ref).abs() <= off + 2.0 ** -11 * (ref.abs() + off) + 2.0 ** -25).all())
