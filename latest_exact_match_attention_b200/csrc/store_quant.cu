@@ -30,9 +30,6 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
-#include <algorithm>
-#include <cstdlib>
-
 #include "store.cuh"
 
 namespace lema {
@@ -459,10 +456,10 @@ int run_quant(QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
 
 template <typename T, int F>
 int run_lanes(QArgs& q, void* ws, size_t ws_bytes, cudaStream_t stream) {
-  // a decode step: store.cu's lanes, but 8 from 8192 items on (int8, 16384 items, load 0.65: 11.4 us with 8 lanes,
-  // 13.2 with 16, 18.0 with 32; 1024 items: 5.9, 4.4, 3.6)
+  // a decode step: store.cu's lanes. Above 8192 items 8 lanes instead of 16 are faster at low loads and lose far more at high
+  // ones, whose chains they walk in twice the round trips (int8, half of the lookups missing, us a layer with 8 / 16 lanes at
+  // loads 0.35, 0.65, 0.9: 8320 items 5.1 / 6.2, 8.0 / 7.2, 59 / 38; 16384 items 7.7 / 11.3, 12.4 / 13.0, 87 / 51).
   int G = q.a.T == 1 ? group_lanes(q.a.n) : 4;
-  if (G == kMidG && q.a.n > kMidMaxItems / 2 && std::getenv("LEMA_K3_GROUP") == nullptr) G = kG;
   while (G < q.chunks) G *= 2;
   if (G == 32) return run_quant<T, F, 32>(q, ws, ws_bytes, stream);
   if (G == 16) return run_quant<T, F, 16>(q, ws, ws_bytes, stream);
