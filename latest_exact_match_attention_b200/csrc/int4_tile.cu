@@ -47,6 +47,8 @@ constexpr int kTileBlocks = kTileRows / 16;       // block rows a tile
 // before it.
 constexpr int kSets = 4;
 
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8};  // CTAs of a cluster that may share a tile's K
+
 // Room for tiles of up to BN tokens.
 template <int BN>
 struct Tile {
@@ -60,6 +62,12 @@ struct Tile {
   static constexpr int kThreads = 32 * (6 + kSets * kSetWarps);
   static constexpr uint32_t kTmemCols = 2 * BN;
   static constexpr int kUnitBytes = 8 * kTileRows * 4;  // 8 tokens of a tile's sums
+  // What a CTA of a split tile receives: the others' sums of its units (256 tokens: 16 units at 2 CTAs, 30 at 6, 28 at 8).
+  static constexpr int exchange_bytes() {
+    int most = 0;
+    for (const int split : kSplits) most = std::max(most, (split - 1) * ((BN / 8 + split - 1) / split) * kUnitBytes);
+    return most;
+  }
   static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + 1024 /* alignment */ + 512 /* barriers */;
 };
 
@@ -522,8 +530,8 @@ __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) tile_kernel(const __gri
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const bool live = warp >= 2 && warp < 6;
     const int mine = (p.bn / 8 + split - 1) / split;  // units of one CTA
-    // where source q's sums of my unit k lie: [q or q - 1][k][two halves of 4 tokens][128 rows]; with at most 32 units
-    // and 8 CTAs that is 28 units of 4 KiB, less than the stages hold
+    // where source q's sums of my unit k lie: [q or q - 1][k][two halves of 4 tokens][128 rows], over the stages
+    // (launch_tile checks that they hold it)
     auto place = [&](int src, int dst, int k) {
       return sbase + static_cast<uint32_t>(((src < dst ? src : src - 1) * mine + k) * TL::kUnitBytes + row_in * 16);
     };
@@ -603,6 +611,7 @@ bool tile_ok(const Args& a, int dtype) {
 
 template <typename T, int BN, bool kGated, bool kSame, bool kSplit>
 int launch_tile(const CUtensorMap& map, const TileArgs& p, int grid, cudaStream_t stream) {
+  static_assert(!kSplit || Tile<BN>::exchange_bytes() <= Tile<BN>::kStages * Tile<BN>::kStageBytes, "the exchange stays inside the stages");
   const auto kernel = tile_kernel<T, BN, kGated, kSame, kSplit>;
   LEMA_TRY(kernel_facts(reinterpret_cast<const void*>(kernel), Tile<BN>::kSmemBytes, 0, 0, nullptr));
   cudaLaunchConfig_t cfg{};
@@ -664,7 +673,7 @@ int choose_shape(TileArgs& p, int sms) {
   for (const int bn : {32, 64, 128, 256}) {
     if (bn > 32 && bn / 2 >= p.a.M) break;  // wider than the rows there are
     const int64_t tiles = ((p.a.M + bn - 1) / bn) * p.f_tiles;
-    for (const int split : {1, 2, 3, 4, 6, 8}) {
+    for (const int split : kSplits) {
       int at_once = sms;
       if (split > 1) {
         if (tiles * split > sms || p.a.n_kb < 3 * split) continue;
