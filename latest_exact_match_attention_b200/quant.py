@@ -120,9 +120,11 @@ class Int4Weight:
     def _lay_out(u, s, n, k, group, gated):
         rb, _, kp = u.shape
         # rows i a (feature 8 i + a); inputs c h t j p e (64 c + 32 h + 8 t + 4 j + 2 p + e)
-        u = u.view(rb, 2, 8, kp // 64, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1).to(torch.int32)
-        shift = torch.arange(8, device=u.device, dtype=torch.int32) * 4         # bits 16 e + 8 p + 4 i
-        words = (u.reshape(rb, kp // 64, 8, 4, 2, 2, 8) << shift).sum(-1, dtype=torch.int32)
+        # each a field of bits 16 e + 8 p + 4 i, one at a time: no 32-bit copy of every code
+        u = u.view(rb, 2, 8, kp // 64, 2, 4, 2, 2, 2).permute(8, 7, 1, 0, 3, 2, 5, 4, 6).reshape(8, -1)
+        words = u[0].to(torch.int32)
+        for field in range(1, 8):
+            words |= u[field].to(torch.int32) << 4 * field
         return Int4Weight(words.view(rb, kp // 64, 32, 4).contiguous(), s.unflatten(1, (2, 8)).permute(0, 3, 2, 1).contiguous(), n, k, group, gated)
 
     def codes(self):

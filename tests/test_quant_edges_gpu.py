@@ -251,3 +251,17 @@ def test_unaligned_rows_through_narrow_weights(cuda, M):
     ref = x.double() @ w.t()
     off = (x.double().abs() @ w.abs().t()) * (K + 8) * 2.0 ** -23
     assert bool(((got.double() - ref).abs() <= off + 2.0 ** -11 * (ref.abs() + off) + 2.0 ** -25).all())
+
+
+def test_packing_needs_a_few_bytes_a_weight(cuda):
+    """The codes themselves are one byte each, the packed weight half a byte."""
+    N, K = 4096, 4096
+    c, s = weight(N, K, 128, BF16, 0, "cpu")
+    c, s = c.to(cuda), s.to(cuda)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    w = Int4Weight.pack(c, s, 128)
+    assert torch.cuda.max_memory_allocated() - base <= 5 * N * K
+    back, _ = w.codes()
+    assert torch.equal(back, c)
