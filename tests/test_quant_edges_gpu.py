@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from latest_exact_match_attention_b200 import quant
-from latest_exact_match_attention_b200._lib import check_status
+from latest_exact_match_attention_b200._lib import call, check_status, device_status, ptr, stream_handle
 from latest_exact_match_attention_b200.cache import HashStore, LemaCache
 from latest_exact_match_attention_b200.model import ModelConfig
 from latest_exact_match_attention_b200.quant import Int4Weight, dequantize_rows, quantize_rows
@@ -265,3 +265,66 @@ def test_packing_needs_a_few_bytes_a_weight(cuda):
     assert torch.cuda.max_memory_allocated() - base <= 5 * N * K
     back, _ = w.codes()
     assert torch.equal(back, c)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("M,N,K,group", [(3, 17, 64, 32), (32, 40, 72, 64), (70, 33, 128, 32), (130, 130, 192, 128), (300, 257, 1096, 64),
+                                         (2500, 1001, 136, 32)])
+def test_values_written_at_odd_offsets_and_strides(cuda, M, N, K, group, dtype, gated):
+    """y inside a larger buffer, off by one element and rows an odd number apart, the residual likewise: the bits of the plain
+    call (the same kernel and tiles), the 64-bit sums within their rounding, and nothing outside y."""
+    (c, s), (c2, s2) = weight(N, K, group, dtype, M, cuda), weight(N, K, group, dtype, M + 1, cuda)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(N)).to(dtype).to(cuda)
+    w = Int4Weight.pack_gate_up(c, s, c2, s2, group) if gated else Int4Weight.pack(c, s, group)
+    wide = N + 2 + (N + 1) % 2                                       # odd
+    room = torch.randn(M + 2, wide, generator=torch.Generator().manual_seed(K)).to(dtype).to(cuda)
+    r = None if gated else room[1: M + 1, 1: N + 1]
+    buf = torch.full((M + 2, wide), 7.0, dtype=dtype, device=cuda)
+    y = buf[1: M + 1, 1: N + 1]
+    tag = {BF16: 1, F16: 2}[dtype]
+    call("lema_int4_linear", ptr(x), tag, M, K, K, ptr(w.packed), ptr(w.scales), tag, group, N, int(gated), ptr(r), wide,
+         y.data_ptr(), wide, ptr(device_status(cuda)), stream_handle(cuda))
+    check_status(cuda)
+    plain = quant.int4_swiglu(x, w) if gated else quant.int4_linear(x, w, r.contiguous())
+    assert torch.equal(y, plain)
+    h = half_step(dtype)
+    a, b = dense64(c, s, group), dense64(c2, s2, group)
+    # a product: fp32 sums of at most K terms (2^-23 each) and half a step a weight
+    off = [(x.double().abs() @ m.abs().t()) * ((K + 8) * 2.0 ** -23 + h) for m in (a, b)]
+    gate, up = x.double() @ a.t(), x.double() @ b.t()
+    if gated:
+        silu = gate * torch.sigmoid(gate)
+        ref = silu * up
+        off = 1.1 * off[0] * (up.abs() + off[1]) + silu.abs() * off[1] + 2.0 ** -17 * ref.abs()
+    else:
+        ref, off = gate + r.double(), off[0] + 2.0 ** -24 * (gate.abs() + r.double().abs())
+    assert bool(((y.double() - ref).abs() <= off + h * (ref.abs() + off) + torch.finfo(dtype).tiny).all())
+    outside = buf.clone()
+    outside[1: M + 1, 1: N + 1] = 7.0
+    assert bool((outside == 7.0).all())
+
+
+@pytest.mark.parametrize("fmt", [None, "int8", "fp8", "int4"])
+@pytest.mark.parametrize("P", [30, 5000, 9000])
+def test_half_steps_at_high_load(cuda, fmt, P):
+    """Lookups then inserts give the rows and entries of the combined step while a table fills to 0.95."""
+    d, steps = 24, 19
+    pair = [HashStore(d, groups=P, dtype=BF16, capacity=20 * P, device=cuda, quant=fmt, segments=3) for _ in range(2)]
+    g = torch.Generator(device=cuda).manual_seed(P)
+    out = [torch.empty(P, d, dtype=BF16, device=cuda) for _ in range(2)]
+    found = 0
+    for t in range(steps):
+        k = torch.full((P,), 977 * t + 5, dtype=torch.int32, device=cuda)              # a new key a step
+        q = (torch.randint(0, max(1, t), (P,), device=cuda, generator=g) * 977 + 5).to(torch.int32)
+        q = torch.where(torch.rand(P, device=cuda, generator=g) < 0.3, q + 1, q)       # absent ones, to the end of their chain
+        v = torch.randn(P, d, device=cuda, generator=g).to(BF16)
+        pair[0].exchange(q, k, v, out[0], 1, 0)
+        out[1].fill_(3.0)
+        pair[1].exchange_phase(q, None, None, out[1], 0, 1)
+        pair[1].exchange_phase(None, k, v, None, 0, 2)
+        assert torch.equal(out[0], out[1])
+        found += int((out[0] != 0).any(1).sum())
+    pair[1].check()
+    assert torch.equal(pair[0].counts, pair[1].counts) and int(pair[0].counts.min()) == steps
+    assert 0.5 * P * (steps - 1) < found < 0.9 * P * steps
