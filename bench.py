@@ -530,6 +530,11 @@ def _model_cfg(which: int, H: int = 64):
     return ModelConfig(vocab_size=50304, depth=24, dim=1536, num_heads=64, d_qk=32, d_v=24)
 
 
+def _quantised(args) -> str:
+    """What --int4 and --rows change, for the record's dtype and metric."""
+    return (f", int4 weights (group {args.int4})" if args.int4 else "") + (f", {args.rows} store rows" if args.rows else "")
+
+
 def run_model_prefill(args):
     """Config 3: full prefill of a random-init 309M-shaped LEMA LM (bf16), B=32 x T=16384
     synthetic tokens, heads swept; every layer runs K1 (codes) and K2 (exact op). One JSON
@@ -547,6 +552,8 @@ def run_model_prefill(args):
         torch.manual_seed(0)
         cfg = _model_cfg(3, H)
         model = Transformer(cfg).to(dev).to(torch.bfloat16).eval()
+        if args.int4:
+            model.quantize_weights_(args.int4)
         for _ in range(max(3, args.warmup)):
             model(idx, return_logits=False)
         torch.cuda.synchronize()
@@ -561,7 +568,8 @@ def run_model_prefill(args):
         print(json.dumps({
             "metric": "LEMA full prefill tokens/s (config 3)", "value": round(Bm * Tm / ms / 1e3, 3),
             "unit": "Mtok/s", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup,
-            "ms_per_step": round(ms, 3), "higher_is_better": True, "dtype": "bf16",
+            "ms_per_step": round(ms, 3), "higher_is_better": True,
+            "dtype": "bf16" + (f", int4 weights (group {args.int4})" if args.int4 else ""),
             "data": "synthetic Zipf(1.1) tokens, 20% bigram copies; random-init weights",
             "config": {"workload": f"cfg3: {cfg.summary()}, B={Bm} T={Tm}", "params": model.n_params()},
             "clocks": clk.summary(),
@@ -578,7 +586,8 @@ def decode_record(args, rank: int, world: int, dev, small: bool = False, worst_l
     sub-record of the headline line (prefix 512, 32 steps). `worst_load`: the stress mode --
     every layer's codes replaced by fresh random codes (cache.worst_case_codes, the reference's
     worst-case hook), the store sized so that it ends at that load. Returns the record (rank 0)
-    with tokens/s of the whole job = all ranks' tokens / max-over-ranks time."""
+    with tokens/s of the whole job = all ranks' tokens / max-over-ranks time. --int4 and --rows (not in the
+    sub-record) serve the model with 4-bit weights and a store of quantised rows."""
     import math
 
     import torch
@@ -587,6 +596,7 @@ def decode_record(args, rank: int, world: int, dev, small: bool = False, worst_l
     from latest_exact_match_attention_b200.cache import worst_case_codes
     from latest_exact_match_attention_b200.decode import decoder
     from latest_exact_match_attention_b200.model import Transformer
+    from latest_exact_match_attention_b200.quant import row_bytes
     cfg = _model_cfg(4)
     B_all = args.decode_batch if worst_load is None else args.worst_batch
     prefix = 512 if small else args.prefix
@@ -597,6 +607,9 @@ def decode_record(args, rank: int, world: int, dev, small: bool = False, worst_l
     Bd = B_all // world
     torch.manual_seed(0)
     model = Transformer(cfg).to(dev).to(torch.bfloat16).eval()
+    int4, fmt, quantised = (0, None, "") if small else (args.int4, args.rows, _quantised(args))
+    if int4:
+        model.quantize_weights_(int4)
     toks = synth.token_stream(B_all, prefix + 1, 50304, seed=0, config_id=4)
     idx = torch.from_numpy(toks[rank * Bd:(rank + 1) * Bd]).to(dev)
     P = Bd * cfg.num_heads
@@ -610,13 +623,14 @@ def decode_record(args, rank: int, world: int, dev, small: bool = False, worst_l
         load = args.max_load
     cap = math.ceil(cfg.depth * P * per_part / load)
     from latest_exact_match_attention_b200 import _lib
-    need = cap * int(_lib.lib().lema_store_slot_bytes(cfg.d_v * 2))
+    held = row_bytes(fmt, cfg.d_v) if fmt else cfg.d_v * 2
+    need = cap * int(_lib.lib().lema_store_slot_bytes(held))
     free = torch.cuda.mem_get_info(dev)[0]
     if need > 0.9 * free - (4 << 30):
         raise SystemExit(f"decode store of {cap} slots ({need / 2**30:.1f} GiB) does not fit the "
                          f"{free / 2**30:.1f} GiB free; lower --entries-per-partition or --decode-batch")
     hook = worst_case_codes(cfg.depth) if worst_load is not None else None
-    cache = model.new_cache("hbm", capacity=cap, batch=Bd, codes_hook=hook)
+    cache = model.new_cache("hbm", capacity=cap, batch=Bd, codes_hook=hook, quant=fmt)
     stream = torch.cuda.current_stream(dev)
 
     def maxr(x):
@@ -649,12 +663,12 @@ def decode_record(args, rank: int, world: int, dev, small: bool = False, worst_l
         torch.cuda.synchronize()
     cache.check()
     ms = maxr(a.elapsed_time(b)) / steps
-    weights = sum(p.numel() * p.element_size() for p in model.parameters())
-    store_bytes = cfg.depth * P * 216          # per (layer, seq, head) op: codes, row, slots
+    weights = sum(t.numel() * t.element_size() for t in (*model.parameters(), *model.buffers()))
+    store_bytes = cfg.depth * P * (120 + 2 * held)   # per (layer, seq, head) op: codes, row in and out, header, held rows
     rec = {
-        "metric": "LEMA batched decode tok/s (config 4)" + (" worst-case codes" if hook else ""),
+        "metric": "LEMA batched decode tok/s (config 4)" + (" worst-case codes" if hook else "") + quantised,
         "value": round(B_all * 1e3 / ms, 1), "unit": "tok/s", "n_gpus": world, "steps": steps,
-        "warmup": warm, "ms_per_step": round(ms, 4), "higher_is_better": True, "dtype": "bf16",
+        "warmup": warm, "ms_per_step": round(ms, 4), "higher_is_better": True, "dtype": "bf16" + quantised,
         "scaling": "strong" if world > 1 else None,
         "data": "synthetic Zipf(1.1) tokens, 20% bigram copies; random-init weights",
         "config": {"workload": f"cfg4: {cfg.summary()}, B={B_all} ({Bd} per GPU), prefix {prefix}",
@@ -1034,6 +1048,9 @@ def main():
     ap.add_argument("--worst-case", action="store_true",
                     help="--workload decode: worst-case codes at store loads 0.5 / 0.9 / 0.95")
     ap.add_argument("--worst-batch", type=int, default=1, help="--workload decode --worst-case: batch")
+    ap.add_argument("--int4", type=int, choices=[0, 32, 64, 128], default=0,
+                    help="--workload decode, model-prefill: 4-bit weights with a scale for this many inputs")
+    ap.add_argument("--rows", choices=["int8", "fp8", "int4"], help="--workload decode: store rows held in 8 or 4 bits")
     ap.add_argument("--no-decode", action="store_true",
                     help="headline line: skip its small batched-decode record")
     ap.add_argument("--heads", type=int, nargs="+", default=[8, 16, 32, 64],
