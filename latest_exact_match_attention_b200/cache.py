@@ -97,6 +97,7 @@ class HashStore:
         self.counts = torch.zeros(groups, dtype=torch.int64, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._ws = None
+        self._ws_stream = 0    # the stream the workspace was allocated on
         # segments > 1: each run of groups/segments groups (a layer, for LemaCache) has its
         # home slots in its own 1/segments of the table; results are the same either way
         segments = max(1, min(int(segments), groups, self.cap))
@@ -125,8 +126,13 @@ class HashStore:
         if torch.cuda.is_current_stream_capturing():
             # the graph's own memory: its replays share it with no other graph or call, and it goes with the graph
             return torch.empty(need, dtype=torch.uint8, device=self.device)
+        stream = stream_handle(self.table.device)
         if self._ws is None or self._ws.numel() < need:
             self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            self._ws_stream = stream
+        elif stream != self._ws_stream:
+            # once a larger one replaces it, its memory is free only when this stream is done with it
+            self._ws.record_stream(torch.cuda.current_stream(self.table.device))
         return self._ws
 
     def exchange(self, qcodes: torch.Tensor, kcodes: torch.Tensor, values: torch.Tensor,

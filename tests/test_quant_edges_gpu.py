@@ -328,3 +328,29 @@ def test_half_steps_at_high_load(cuda, fmt, P):
     pair[1].check()
     assert torch.equal(pair[0].counts, pair[1].counts) and int(pair[0].counts.min()) == steps
     assert 0.5 * P * (steps - 1) < found < 0.9 * P * steps
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_a_replaced_workspace_is_not_handed_out_while_another_stream_uses_it(cuda, fmt):
+    P, T, d = 8, 2048, 16
+    st = HashStore(d, groups=P, dtype=BF16, capacity=400000, device=cuda, quant=fmt)
+
+    def items(t):
+        k = torch.arange(P * t, dtype=torch.int32, device=cuda)
+        return k, k, torch.zeros(P * t, d, dtype=BF16, device=cuda), torch.empty(P * t, d, dtype=BF16, device=cuda), t, 0
+    small, large = items(T), items(4 * T)
+    st.exchange(*small)
+    old, size = st._ws.data_ptr(), st._ws.numel()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)                    # some 50 ms: the exchanges below are still to come
+        st.exchange(*small, check=False)
+        st.exchange(*large, check=False)
+    assert st._ws.data_ptr() != old
+    again = torch.empty(size, dtype=torch.uint8, device=cuda)
+    assert again.data_ptr() != old
+    torch.cuda.synchronize()
+    st.check()
+    # partition p: codes p T ... of the small calls, 4 p T ... of the large one; shared in partition 0 alone
+    assert len(st) == P * 4 * T + (P - 1) * T
