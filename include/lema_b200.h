@@ -457,7 +457,7 @@ int lema_ipc_close(void* ptr, int64_t offset);
  *   residual, y  [M] rows of N values of `dtype`, ldr / ldy elements apart; residual may be NULL or y
  * gated != 0: the block rows hold 8 gate features (i = 0) and the 8 up features of the same indices
  * (i = 1), N counts the features of each, and y = silu(gate) * up with both sums in fp32 (ceil(N / 8)
- * block rows; no residual). Sums are fp32, rounded once to dtype; fp32 inputs keep fp32 accuracy. Up to 32
+ * block rows; no residual). Sums are fp32, rounded once to dtype; fp32 inputs keep fp32 accuracy (a group's sum of x * q has to stay within fp32: |x| < 2^118). Up to 32
  * rows, and rows that TMA cannot read (K < 64, ldx or x not a multiple of 16 bytes), multiply the codes
  * exactly and scale each group's fp32 sum; more 16-bit rows multiply s * q rounded once to dtype's significant bits.
  * (fp16's range does not bound s * q: a feature's weights are held times a power of two that its largest scale sets, so

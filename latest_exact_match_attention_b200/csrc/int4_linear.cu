@@ -17,7 +17,7 @@
 // so that the card is full of warps: a token through a 1536 x 1536 projection has 96 block rows and takes 16
 // warps for each, the vocabulary's 3144 block rows one each. What bounds the small calls is the latency of a
 // few dependent loads, so every warp keeps kDeep blocks (words, scales and inputs) in flight in registers; the large
-// ones are bound by the instructions issued, about 70 a block of 1024 weights where rows are whole (kWhole: K a
+// ones are bound by the instructions issued, about 106 a block of 1024 weights where rows are whole (kWhole: K a
 // multiple of 64, 16-byte aligned rows, so that no load is checked; rows past the last read the last again, and
 // what they give is dropped). A ring in shared memory (cp.async) instead of registers was no faster.
 #include <cuda_bf16.h>

@@ -1,5 +1,5 @@
-// Products of many rows with 4-bit weights (int4_linear.cu's definition; prompts and large decode batches):
-// bound by the tensor cores, 2 M N K operations. One persistent CTA per SM walks tiles of 128 weight rows
+// Products of many rows with 4-bit weights (int4_linear.cu's definition; prompts and large decode batches).
+// The floor is the tensor cores' 2 M N K operations; bound by the dequantisation (below). One persistent CTA per SM walks tiles of 128 weight rows
 // (features) x BN tokens, features on the M side of tcgen05.mma so that the weights' fragment layout is
 // also this kernel's and a small batch needs no padding to 128 rows. Warp roles:
 //   warp 0      TMA producer: BN x 64 tiles of x (128-byte swizzle) into a ring of stages;
