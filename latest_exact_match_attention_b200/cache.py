@@ -93,7 +93,8 @@ class HashStore:
         self.stride = int(_lib.lib().lema_store_slot_bytes(self.vbytes))
         self.cap = max(16, int(capacity))
         self.table = torch.zeros((self.cap, self.stride), dtype=torch.uint8, device=self.device)
-        self._index = self.table.device.index
+        self.device = self.table.device      # "cuda" alone would mean whichever device is current at a later call
+        self._index = self.device.index
         self.counts = torch.zeros(groups, dtype=torch.int64, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._ws = None
@@ -126,13 +127,13 @@ class HashStore:
         if torch.cuda.is_current_stream_capturing():
             # the graph's own memory: its replays share it with no other graph or call, and it goes with the graph
             return torch.empty(need, dtype=torch.uint8, device=self.device)
-        stream = stream_handle(self.table.device)
+        stream = stream_handle(self.device)
         if self._ws is None or self._ws.numel() < need:
             self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             self._ws_stream = stream
         elif stream != self._ws_stream:
             # once a larger one replaces it, its memory is free only when this stream is done with it
-            self._ws.record_stream(torch.cuda.current_stream(self.table.device))
+            self._ws.record_stream(torch.cuda.current_stream(self.device))
         return self._ws
 
     def exchange(self, qcodes: torch.Tensor, kcodes: torch.Tensor, values: torch.Tensor,

@@ -354,3 +354,12 @@ def test_a_replaced_workspace_is_not_handed_out_while_another_stream_uses_it(cud
     st.check()
     # partition p: codes p T ... of the small calls, 4 p T ... of the large one; shared in partition 0 alone
     assert len(st) == P * 4 * T + (P - 1) * T
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_a_store_stays_on_the_device_it_was_made_on(cuda, fmt):
+    """Its workspace and streams too: the device it was given without an index is the one current then."""
+    st = HashStore(16, groups=4, dtype=BF16, device="cuda", quant=fmt)
+    assert st.device == st.table.device and st.device.index == torch.cuda.current_device()
+    cache = LemaCache(ModelConfig(vocab_size=128, depth=1, dim=64, num_heads=4, d_qk=32, d_v=16), device="cuda", quant=fmt)
+    assert cache.store.device.index is not None
