@@ -315,6 +315,8 @@ class LayerStore:
         # which is the item order the store takes
         if self.buffers.codes_hook is not None:
             qc, kc = self.buffers.codes_hook(self.g0 // self.partitions, qc, kc)
+        if kc.dtype != qc.dtype:
+            kc = kc.to(qc.dtype)        # one width: a negative int32 and the int64 of its value are other 64-bit codes
         n, d_v = qc.numel(), v.shape[-1]
         T = n // self.partitions
         if T > 1 and not self.persistent_out and v.dim() == 4 and v.stride(-1) == 1:

@@ -363,3 +363,17 @@ def test_a_store_stays_on_the_device_it_was_made_on(cuda, fmt):
     assert st.device == st.table.device and st.device.index == torch.cuda.current_device()
     cache = LemaCache(ModelConfig(vocab_size=128, depth=1, dim=64, num_heads=4, d_qk=32, d_v=16), device="cuda", quant=fmt)
     assert cache.store.device.index is not None
+
+
+@pytest.mark.parametrize("quant", [None, "int8"])
+def test_half_steps_take_key_codes_of_the_other_width(cuda, quant):
+    cfg = ModelConfig(vocab_size=128, depth=1, dim=64, num_heads=4, d_qk=32, d_v=16)
+    c = [LemaCache(cfg, dtype=BF16, batch=1, max_cache_len=40, device=cuda, quant=quant) for _ in range(2)]
+    g = torch.Generator().manual_seed(3)
+    for _ in range(20):
+        q, k = ((torch.randint(0, 5, (1, 4, 1), generator=g) - 3).to(torch.int32).to(cuda) for _ in range(2))
+        v = torch.randn(1, 4, 1, 16, generator=g).to(BF16).to(cuda)
+        s, got = c[1].layer(0).lookup(q, k.long(), v)
+        c[1].layer(0).insert(s)
+        assert torch.equal(c[0].layer(0).exchange(q, k, v), got)
+    assert torch.equal(c[0].counts(), c[1].counts())
